@@ -46,6 +46,15 @@ _SIGNATURES = {
     "acache_linear_argmax_scratch_bytes": (c_int64, [c_int, c_int]),
     "acache_linear_argmax": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p,
                                      c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "acache_quantize_rows": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "acache_rmsnorm_int8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_float, c_int,
+                                    c_void_p, c_void_p, c_void_p]),
+    "acache_act_mul_halves_int8": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "acache_linear_int8": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                   c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "acache_rope_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int,
+                                   c_int, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_int64, c_void_p,
+                                   c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "acache_diag_mma_rate": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
     "acache_anchor_topk": (c_int, [c_void_p, c_int, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "acache_anchor_importance_scratch_bytes": (c_int64, [c_int, c_int, c_int]),
@@ -124,6 +133,23 @@ def ptr(t: torch.Tensor | None):
 
 def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device_of(t: torch.Tensor):
+    """``with on_device_of(t): launch`` - makes the tensor's device current for the launch (its current
+    stream, its context) when it is not."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 # kernels launched through this binding since import (the benchmark reads the difference)

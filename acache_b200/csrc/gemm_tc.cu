@@ -12,6 +12,8 @@
 //            its fp32 sums in partial[s]; for projections with so few output tiles that whole
 //            tiles would leave most of the 74 pairs idle.  The normalisation kernel that consumes
 //            the projection adds the slices (`acache_add_rmsnorm_partials`).
+//   int8     X and W hold 8-bit integers, the sums are 32-bit integers (exact), and
+//            out[i, j] = acc * x_scale[i] * w_scale[j] (+ bias) in fp32, rounded once
 //
 // Two CTAs of a cluster work as one: `tcgen05.mma.cta_group::2` multiplies a 256-row block of X
 // (128 rows staged by each CTA) with a BN-column block of W (BN/2 rows staged by each CTA), so a
@@ -42,7 +44,7 @@ constexpr int kPairs = kNumSMs / 2;
 constexpr int kMaxStages = 8;
 constexpr uint32_t kTmemCols = 512;
 
-enum { EPI_PLAIN = 0, EPI_SWIGLU = 1, EPI_QKV = 2, EPI_ARGMAX = 3, EPI_PARTIAL = 4 };
+enum { EPI_PLAIN = 0, EPI_SWIGLU = 1, EPI_QKV = 2, EPI_ARGMAX = 3, EPI_PARTIAL = 4, EPI_INT8 = 5 };
 
 struct Params {
   int M, N, K, MB, BN, stages, acc_stages, group;
@@ -56,6 +58,8 @@ struct Params {
   // argmax: per (column tile, row) partial maximum, its column and the sum of exp(x - maximum)
   float* part_max; int32_t* part_arg; float* part_sum;
   int32_t* err_flag;
+  // int8: one scale per row of X and per row of W
+  const float* x_scale; const float* w_scale;
 };
 
 // TMA tile load of this CTA's half of a pair's operand; the bytes are counted on `bar`, which
@@ -65,56 +69,58 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
 }
-// All products of one k block of the pair (4 k steps of 16 x MB row blocks) from ONE statement, so
+// All products of one k block of the pair (4 k steps of 32 bytes x MB row blocks) from ONE statement, so
 // that the issuing thread spends a few integer operations per product: the operand descriptors
 // differ only in their 14-bit start address, which advances by 2 (32 bytes) per k step and by 1024
 // (16 KB) per row block.  `hi` is the descriptors' common upper word, `a_lo` / `b_lo` the lower
 // words for k step 0; `first` = 0 starts the accumulators over with the first k step.
-#define ACACHE_MMA2 "tcgen05.mma.cta_group::2.kind::f16 "
-template <int MB>
+#define ACACHE_KBLOCK1(MMA)                                                                                      \
+  asm volatile(                                                                                                  \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 ta, tb;\n\t"                                       \
+      "setp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 q, %5, %5;\n\t"                                                     \
+      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"                                                      \
+      MMA "[%0], da, db, %4, p;\n\t"                                                                            \
+      "add.u32 ta, %1, 2;\n\tadd.u32 tb, %2, 2;\n\tmov.b64 da, {ta, %3};\n\tmov.b64 db, {tb, %3};\n\t"          \
+      MMA "[%0], da, db, %4, q;\n\t"                                                                            \
+      "add.u32 ta, %1, 4;\n\tadd.u32 tb, %2, 4;\n\tmov.b64 da, {ta, %3};\n\tmov.b64 db, {tb, %3};\n\t"          \
+      MMA "[%0], da, db, %4, q;\n\t"                                                                            \
+      "add.u32 ta, %1, 6;\n\tadd.u32 tb, %2, 6;\n\tmov.b64 da, {ta, %3};\n\tmov.b64 db, {tb, %3};\n\t"          \
+      MMA "[%0], da, db, %4, q;\n\t}"                                                                           \
+      ::"r"(d0), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(first) : "memory")
+#define ACACHE_KBLOCK2(MMA)                                                                                      \
+  asm volatile(                                                                                                  \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, dc, db;\n\t.reg .b32 ta, tc, tb;\n\t"                               \
+      "setp.ne.b32 p, %6, 0;\n\tsetp.eq.b32 q, %6, %6;\n\t"                                                     \
+      "add.u32 tc, %2, 1024;\n\tmov.b64 da, {%2, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {%3, %4};\n\t"    \
+      MMA "[%0], da, db, %5, p;\n\t"                                                                            \
+      MMA "[%1], dc, db, %5, p;\n\t"                                                                            \
+      "add.u32 ta, %2, 2;\n\tadd.u32 tc, %2, 1026;\n\tadd.u32 tb, %3, 2;\n\t"                                   \
+      "mov.b64 da, {ta, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {tb, %4};\n\t"                             \
+      MMA "[%0], da, db, %5, q;\n\t"                                                                            \
+      MMA "[%1], dc, db, %5, q;\n\t"                                                                            \
+      "add.u32 ta, %2, 4;\n\tadd.u32 tc, %2, 1028;\n\tadd.u32 tb, %3, 4;\n\t"                                   \
+      "mov.b64 da, {ta, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {tb, %4};\n\t"                             \
+      MMA "[%0], da, db, %5, q;\n\t"                                                                            \
+      MMA "[%1], dc, db, %5, q;\n\t"                                                                            \
+      "add.u32 ta, %2, 6;\n\tadd.u32 tc, %2, 1030;\n\tadd.u32 tb, %3, 6;\n\t"                                   \
+      "mov.b64 da, {ta, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {tb, %4};\n\t"                             \
+      MMA "[%0], da, db, %5, q;\n\t"                                                                            \
+      MMA "[%1], dc, db, %5, q;\n\t}"                                                                           \
+      ::"r"(d0), "r"(d1), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(first) : "memory")
+template <int MB, bool I8>
 __device__ __forceinline__ void issue_kblock(uint32_t d0, uint32_t d1, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
-                                             uint32_t idesc, uint32_t first);
-template <>
-__device__ __forceinline__ void issue_kblock<1>(uint32_t d0, uint32_t d1, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
-                                                uint32_t idesc, uint32_t first) {
-  (void)d1;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t.reg .b32 ta, tb;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 q, %5, %5;\n\t"
-      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %4, p;\n\t"
-      "add.u32 ta, %1, 2;\n\tadd.u32 tb, %2, 2;\n\tmov.b64 da, {ta, %3};\n\tmov.b64 db, {tb, %3};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %4, q;\n\t"
-      "add.u32 ta, %1, 4;\n\tadd.u32 tb, %2, 4;\n\tmov.b64 da, {ta, %3};\n\tmov.b64 db, {tb, %3};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %4, q;\n\t"
-      "add.u32 ta, %1, 6;\n\tadd.u32 tb, %2, 6;\n\tmov.b64 da, {ta, %3};\n\tmov.b64 db, {tb, %3};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %4, q;\n\t}"
-      ::"r"(d0), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(first) : "memory");
+                                             uint32_t idesc, uint32_t first) {
+  if constexpr (MB == 1) {
+    (void)d1;
+    if constexpr (I8) ACACHE_KBLOCK1("tcgen05.mma.cta_group::2.kind::i8 ");
+    else ACACHE_KBLOCK1("tcgen05.mma.cta_group::2.kind::f16 ");
+  } else {
+    if constexpr (I8) ACACHE_KBLOCK2("tcgen05.mma.cta_group::2.kind::i8 ");
+    else ACACHE_KBLOCK2("tcgen05.mma.cta_group::2.kind::f16 ");
+  }
 }
-template <>
-__device__ __forceinline__ void issue_kblock<2>(uint32_t d0, uint32_t d1, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
-                                                uint32_t idesc, uint32_t first) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, dc, db;\n\t.reg .b32 ta, tc, tb;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\tsetp.eq.b32 q, %6, %6;\n\t"
-      "add.u32 tc, %2, 1024;\n\tmov.b64 da, {%2, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {%3, %4};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %5, p;\n\t"
-      ACACHE_MMA2 "[%1], dc, db, %5, p;\n\t"
-      "add.u32 ta, %2, 2;\n\tadd.u32 tc, %2, 1026;\n\tadd.u32 tb, %3, 2;\n\t"
-      "mov.b64 da, {ta, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {tb, %4};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %5, q;\n\t"
-      ACACHE_MMA2 "[%1], dc, db, %5, q;\n\t"
-      "add.u32 ta, %2, 4;\n\tadd.u32 tc, %2, 1028;\n\tadd.u32 tb, %3, 4;\n\t"
-      "mov.b64 da, {ta, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {tb, %4};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %5, q;\n\t"
-      ACACHE_MMA2 "[%1], dc, db, %5, q;\n\t"
-      "add.u32 ta, %2, 6;\n\tadd.u32 tc, %2, 1030;\n\tadd.u32 tb, %3, 6;\n\t"
-      "mov.b64 da, {ta, %4};\n\tmov.b64 dc, {tc, %4};\n\tmov.b64 db, {tb, %4};\n\t"
-      ACACHE_MMA2 "[%0], da, db, %5, q;\n\t"
-      ACACHE_MMA2 "[%1], dc, db, %5, q;\n\t}"
-      ::"r"(d0), "r"(d1), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(first) : "memory");
-}
-#undef ACACHE_MMA2
+#undef ACACHE_KBLOCK1
+#undef ACACHE_KBLOCK2
 
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile int* abort) {
   const long long t0 = clock64();
@@ -191,6 +197,27 @@ __device__ __forceinline__ void epi_partial(const Params& p, int ks, int m, int 
   for (int i = 0; i < 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
 
+// 32-bit integer sums, the two scales applied one after the other in fp32 (their product could leave
+// the range of fp32 where the result does not)
+template <typename T>
+__device__ __forceinline__ void epi_int8(const Params& p, int m, int n, const uint32_t* v, float x_scale) {
+  float o[16], ws[16];
+  load8<float>(p.w_scale + n, ws);
+  load8<float>(p.w_scale + n + 8, ws + 8);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = ((float)(int32_t)v[i] * x_scale) * ws[i];
+  if (p.bias) {
+    float b[16];
+    load8<T>((const T*)p.bias + n, b);
+    load8<T>((const T*)p.bias + n + 8, b + 8);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] += b[i];
+  }
+  T* dst = (T*)p.out + (int64_t)m * p.ldo + n;
+  *reinterpret_cast<uint4*>(dst) = pack8<T>(o);
+  *reinterpret_cast<uint4*>(dst + 8) = pack8<T>(o + 8);
+}
+
 // W rows are interleaved in groups of 8: columns n..n+7 are gate features n/2..n/2+7 and columns
 // n+8..n+15 the up features of the same indices; both projections are rounded to T first, the
 // activation is rounded to T, then the product, as the separate kernels do
@@ -264,10 +291,13 @@ __device__ __forceinline__ void epi_qkv(const Params& p, int m, int n, const flo
   }
 }
 
+// T: operand type (int8_t: TR is the output type); TR, TC: RoPE table and arithmetic types of EPI_QKV
 template <typename T, typename TR, typename TC, int EPI, int MB>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NT, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                  const __grid_constant__ Params p) {
+  constexpr bool I8 = EPI == EPI_INT8;
+  constexpr int BKE = 128 / (int)sizeof(T);    // elements of a k block: 128 bytes of every row
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   chain_release();
   const int BN = p.BN, S = p.stages, AS = p.acc_stages;
@@ -292,7 +322,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   const int n_tiles = (p.N + BN - 1) / BN;
   const int mn_tiles = m_tiles * n_tiles;
   const int total = mn_tiles * p.ksplit;       // slice-major: the slices of a tile run on different pairs
-  const int k_blocks = (p.K + BK - 1) / BK;
+  const int k_blocks = (p.K + BKE - 1) / BKE;
   const int k_per = (k_blocks + p.ksplit - 1) / p.ksplit;   // the host made sure no slice is empty
   const int acc_cols = (BN + 31) & ~31;       // TMEM columns reserved per accumulator
 
@@ -339,15 +369,17 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
           if (rank == 0) mbar_expect_tx(bar(FULL + s), (uint32_t)(2 * stage_bytes));   // both CTAs' bytes
           const uint32_t full = map_to_cta(bar(FULL + s), 0);
           const uint32_t dst = smem_u32(ring) + s * stage_bytes;
-          for (int r = 0; r < MB; ++r) tma_load_2d_pair(dst + r * A_SUB, &tmap_x, full, kb * BK, m0 + r * 256);
-          tma_load_2d_pair(dst + MB * A_SUB, &tmap_w, full, kb * BK, n0);
+          for (int r = 0; r < MB; ++r) tma_load_2d_pair(dst + r * A_SUB, &tmap_x, full, kb * BKE, m0 + r * 256);
+          tma_load_2d_pair(dst + MB * A_SUB, &tmap_w, full, kb * BKE, n0);
         }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ product issuer (leader CTA)
     if (lane == 0 && rank == 0 && !*abort_flag) {
-      const uint32_t idesc = make_idesc(Fmt<T>::id, 0, (uint32_t)BN, 256);
+      uint32_t idesc;
+      if constexpr (I8) idesc = make_idesc_i8((uint32_t)BN, 256);
+      else idesc = make_idesc(Fmt<T>::id, 0, (uint32_t)BN, 256);
       // descriptor words: start address in 16-byte units | leading offset 16 B; stride 1024 B between
       // 8-row groups, descriptor version, 128-byte swizzle
       const uint32_t desc_hi = 64u | (1u << 14) | (2u << 29);
@@ -368,7 +400,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
           if (!ok) break;
           tc_fence_after();
           const uint32_t a_lo = ring_lo + (uint32_t)s * stage_units;
-          issue_kblock<MB>(d0, d1, a_lo, a_lo + b_units, desc_hi, idesc, kb > kb_begin ? 1u : 0u);
+          issue_kblock<MB, I8>(d0, d1, a_lo, a_lo + b_units, desc_hi, idesc, kb > kb_begin ? 1u : 0u);
           // the group of stages is free in both CTAs once these products have read it
           if ((s & (G - 1)) == G - 1) mma_commit_pair(bar(EMPTY + s / G));
           if (++s == S) {
@@ -417,6 +449,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
             slot = -1;
           }
         }
+        float row_scale = 0.f;
+        if (I8 && live) row_scale = p.x_scale[m];
         float run_max = -INFINITY, run_sum = 0.f;
         int run_arg = 0;
 #pragma unroll 1
@@ -432,11 +466,12 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
             if (half == 1 && !two) break;
             const float* v = reinterpret_cast<const float*>(half == 0 ? v0 : v1);
             const int nn = n0 + c + half * 16;
-            if (EPI == EPI_PLAIN) epi_plain<T>(p, m, nn, v);
-            if (EPI == EPI_PARTIAL) epi_partial(p, ks, m, nn, v);
-            if (EPI == EPI_SWIGLU) epi_swiglu<T>(p, m, nn, v);
-            if (EPI == EPI_QKV) epi_qkv<T, TR, TC>(p, m, nn, v, pos, slot);
-            if (EPI == EPI_ARGMAX) {
+            if constexpr (EPI == EPI_PLAIN) epi_plain<T>(p, m, nn, v);
+            if constexpr (EPI == EPI_PARTIAL) epi_partial(p, ks, m, nn, v);
+            if constexpr (EPI == EPI_SWIGLU) epi_swiglu<T>(p, m, nn, v);
+            if constexpr (EPI == EPI_QKV) epi_qkv<T, TR, TC>(p, m, nn, v, pos, slot);
+            if constexpr (EPI == EPI_INT8) epi_int8<TR>(p, m, nn, half == 0 ? v0 : v1, row_scale);
+            if constexpr (EPI == EPI_ARGMAX) {
               // logits as the unfused projection leaves them (rounded to T); first maximum wins
               float x[16], mx = -INFINITY;
               int am = 0;
@@ -763,4 +798,34 @@ extern "C" int acache_linear_argmax(const void* x, int64_t x_stride, int n_rows,
                                                              x0, confidence);
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;
+}
+
+extern "C" int acache_linear_int8(const int8_t* x, int64_t x_stride, const float* x_scale, int n_rows, int in_features,
+                                  const int8_t* weight, const float* w_scale, int out_features, const void* bias, int dtype,
+                                  void* out, int64_t out_stride, int tile_mb, int tile_bn, int32_t* err_flag, void* stream) {
+  if (n_rows < 0 || in_features <= 0 || out_features <= 0) return ACACHE_EINVAL;
+  if (dtype != ACACHE_BF16 && dtype != ACACHE_F16) return ACACHE_EUNSUPPORTED;
+  if (n_rows == 0) return ACACHE_OK;
+  if (!x || !x_scale || !weight || !w_scale || !out) return ACACHE_EINVAL;
+  if (in_features % 16 != 0 || out_features % 16 != 0 || x_stride % 16 != 0 || out_stride % 8 != 0 || !aligned16(x) ||
+      !aligned16(weight) || !aligned16(w_scale) || !aligned16(out) || (bias && !aligned16(bias)))
+    return ACACHE_EUNSUPPORTED;
+  // |acc| <= 128 * 128 * K has to fit 31 bits
+  if (in_features > 131071) return ACACHE_ELIMIT;
+  if ((tile_mb != 0 && tile_mb != 1 && tile_mb != 2) || (tile_bn != 0 && (tile_bn % 32 != 0 || tile_bn < 64 || tile_bn > 256)))
+    return ACACHE_EINVAL;
+  const gemm::Tile tile = gemm::pick_tile(n_rows, out_features, tile_mb, tile_bn, 32, 1.03);
+  if (tile.smem == 0) return ACACHE_EUNSUPPORTED;
+  gemm::Params p{};
+  p.M = n_rows; p.N = out_features; p.K = in_features; p.MB = tile.mb; p.BN = tile.bn; p.stages = tile.stages;
+  p.acc_stages = tile.acc_stages; p.ksplit = 1; p.group = tile.mb == 1 ? 2 : 1;
+  if (p.group == 2 && (p.stages & 1)) p.stages -= 1;
+  CUtensorMap mx, mw;
+  if (!tc::make_tensor_map_2d_i8(&mx, x, n_rows, in_features, x_stride, 128) ||
+      !tc::make_tensor_map_2d_i8(&mw, weight, out_features, in_features, in_features, tile.bn / 2))
+    return ACACHE_EUNSUPPORTED;
+  p.out = out; p.ldo = out_stride; p.bias = bias; p.err_flag = err_flag; p.x_scale = x_scale; p.w_scale = w_scale;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == ACACHE_BF16) return gemm::launch<int8_t, __nv_bfloat16, float, gemm::EPI_INT8>(mx, mw, p, tile, st);
+  return gemm::launch<int8_t, __half, float, gemm::EPI_INT8>(mx, mw, p, tile, st);
 }

@@ -1,0 +1,253 @@
+// Rows quantised to 8-bit integers by the kernel that produces them (input side of the 8-bit
+// projections in gemm_i8.cu):
+//
+//   a_i = max_k |y_ik|      q_ik = round(127 y_ik / a_i), ties to even      scale_i = a_i / 127
+//
+// where y is the row itself, its RMSNorm (with the residual add before it), or act(gate) * up of a
+// row that holds both halves.  y stays in fp32 registers from the producer to the rounding: it is
+// never rounded to the model type in between, which the unfused chain does.
+//
+// The quotient t = 127 y / a is formed as y * (127 / a), which is within 2 units of its last place, and
+// its 24 significant bits are rounded to 21.  For 16-bit y and a with significands Y, A < 2^11 the exact
+// t lies on a tie k + 1/2 or at least t / (254 Y) > 2^-19 t from one (the difference is a whole number of
+// units of y's last place over 2a), so rounding to 21 bits restores exact ties and moves nothing else
+// across one: 16-bit rows are quantised as by exact division, at the price of a multiplication.
+//
+// A row that holds an infinity or a NaN gets the scale NaN and zeros, so that everything computed
+// from it is NaN; a row of zeros gets the scale 0.
+//
+// One CTA per row, one pass over global memory (the row stays in registers); bound by HBM, in
+// practice by latency at the few hundred rows of a decode step.
+#include "common.cuh"
+
+namespace acache {
+namespace quant {
+
+enum { SRC_ROWS = 0, SRC_NORM = 1, SRC_GATE = 2 };
+
+struct Params {
+  const void* x; int64_t x_stride; const void* delta; int64_t d_stride; const void* weight; float eps; int act;
+  int8_t* q; float* scale; int n_cols;
+};
+
+__device__ __forceinline__ float act_fn(float x, int act) {
+  if (act == 0) return x / (1.f + expf(-x));
+  if (act == 1) return fmaxf(x, 0.f);
+  return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+}
+
+// largest |v| as ordered bits: a NaN is larger than an infinity, which is larger than any number
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+struct RowScale { float pre, f; bool dead; };   // q = round((v * pre) * f)
+
+__device__ __forceinline__ RowScale row_scale(uint32_t top_bits, float* scale_out) {
+  RowScale r;
+  const float top = __uint_as_float(top_bits);
+  const bool finite = top_bits < 0x7F800000u;
+  r.pre = top < 0x1p-100f ? 0x1p100f : 1.f;     // keeps 127 / a inside the range of fp32
+  r.dead = !finite || top == 0.f;
+  r.f = r.dead ? 0.f : 127.f / (top * r.pre);
+  if (scale_out) *scale_out = finite ? top / 127.f : __uint_as_float(0x7FC00000u);
+  return r;
+}
+
+__device__ __forceinline__ int quantise(float v, const RowScale& r) {
+  float t = (v * r.pre) * r.f;
+  t = __uint_as_float((__float_as_uint(t) + 4u) & ~7u);     // 21 significant bits
+  const int q = (int)(__float_as_uint(t + 0x1.8p23f) & 0xFFu);
+  return r.dead ? 0 : q;
+}
+
+template <int NT>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
+  v = __reduce_max_sync(0xFFFFFFFFu, v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) m = max(m, red[i]);
+  return m;
+}
+
+template <int NT>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) s += red[i];
+  return s;
+}
+
+template <typename T, int SRC, int NT, int VPT>
+__global__ void __launch_bounds__(NT) quantise_kernel(const Params p) {
+  constexpr int E = 16 / sizeof(T);
+  chain_release();
+  chain_wait();
+  __shared__ float red_sum[NT / 32];
+  __shared__ uint32_t red_max[NT / 32];
+  const int64_t row = blockIdx.x;
+  T* xr = (T*)p.x + row * p.x_stride;
+  const int nvec = p.n_cols / E;
+  float y[VPT][E];
+  uint32_t top = 0;
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = threadIdx.x + i * NT;
+    if (c < nvec) {
+      Vec16<T> a;
+      a.u = *reinterpret_cast<const uint4*>(xr + (int64_t)c * E);
+      if (SRC == SRC_NORM && p.delta) {           // the residual add, rounded to T, written back
+        Vec16<T> b;
+        b.u = ld_global_nc((const T*)p.delta + row * p.d_stride + (int64_t)c * E);
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.e[e] = from_f32<T>(to_f32<T>(a.e[e]) + to_f32<T>(b.e[e]));
+        *reinterpret_cast<uint4*>(xr + (int64_t)c * E) = a.u;
+      }
+      if (SRC == SRC_GATE) {
+        Vec16<T> b;
+        b.u = *reinterpret_cast<const uint4*>(xr + p.n_cols + (int64_t)c * E);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[i][e] = act_fn(to_f32<T>(a.e[e]), p.act) * to_f32<T>(b.e[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          y[i][e] = to_f32<T>(a.e[e]);
+          if (SRC == SRC_NORM) ss = fmaf(y[i][e], y[i][e], ss);
+        }
+      }
+      if (SRC != SRC_NORM) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = max(top, abs_bits(y[i][e]));
+      }
+    }
+  }
+  if (SRC == SRC_NORM) {
+    const float rs = rsqrtf(block_sum<NT>(ss, red_sum) / (float)p.n_cols + p.eps);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = threadIdx.x + i * NT;
+      if (c < nvec) {
+        Vec16<T> w;
+        w.u = *reinterpret_cast<const uint4*>((const T*)p.weight + (int64_t)c * E);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          y[i][e] = y[i][e] * rs * to_f32<T>(w.e[e]);
+          top = max(top, abs_bits(y[i][e]));
+        }
+      }
+    }
+  }
+  top = block_max<NT>(top, red_max);
+  const RowScale r = row_scale(top, threadIdx.x == 0 ? p.scale + row : nullptr);
+  int8_t* qr = p.q + row * p.n_cols;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = threadIdx.x + i * NT;
+    if (c < nvec) {
+      uint32_t w[E / 4];
+#pragma unroll
+      for (int g = 0; g < E / 4; ++g) {
+        w[g] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[g] |= (uint32_t)quantise(y[i][4 * g + e], r) << (8 * e);
+      }
+      if (E == 8) *reinterpret_cast<uint2*>(qr + (int64_t)c * E) = make_uint2(w[0], w[E / 4 - 1]);
+      else *reinterpret_cast<uint32_t*>(qr + (int64_t)c * E) = w[0];
+    }
+  }
+}
+
+// any width, alignment and stride: one element per thread and step, the row read again per phase
+template <typename T, int SRC>
+__global__ void __launch_bounds__(256) quantise_any_kernel(const Params p) {
+  chain_release();
+  chain_wait();
+  __shared__ float red_sum[8];
+  __shared__ uint32_t red_max[8];
+  const int64_t row = blockIdx.x;
+  T* xr = (T*)p.x + row * p.x_stride;
+  float ss = 0.f, rs = 0.f;
+  if (SRC == SRC_NORM) {
+    for (int c = threadIdx.x; c < p.n_cols; c += 256) {
+      float v = to_f32<T>(xr[c]);
+      if (p.delta) {
+        const T s = from_f32<T>(v + to_f32<T>(((const T*)p.delta)[row * p.d_stride + c]));
+        xr[c] = s;                                  // read back by this thread only
+        v = to_f32<T>(s);
+      }
+      ss = fmaf(v, v, ss);
+    }
+    rs = rsqrtf(block_sum<256>(ss, red_sum) / (float)p.n_cols + p.eps);
+  }
+  auto value = [&](int c) {
+    const float v = to_f32<T>(xr[c]);
+    if (SRC == SRC_NORM) return v * rs * to_f32<T>(((const T*)p.weight)[c]);
+    if (SRC == SRC_GATE) return act_fn(v, p.act) * to_f32<T>(xr[p.n_cols + c]);
+    return v;
+  };
+  uint32_t top = 0;
+  for (int c = threadIdx.x; c < p.n_cols; c += 256) top = max(top, abs_bits(value(c)));
+  top = block_max<256>(top, red_max);
+  const RowScale r = row_scale(top, threadIdx.x == 0 ? p.scale + row : nullptr);
+  int8_t* qr = p.q + row * p.n_cols;
+  for (int c = threadIdx.x; c < p.n_cols; c += 256) qr[c] = (int8_t)quantise(value(c), r);
+}
+
+template <typename T, int SRC>
+static int launch(const Params& p, int64_t n_rows, cudaStream_t st) {
+  constexpr int E = 16 / sizeof(T);
+  const bool vec = p.n_cols % E == 0 && p.x_stride % E == 0 && aligned16(p.x) && (!p.delta || (p.d_stride % E == 0 && aligned16(p.delta))) &&
+                   (!p.weight || aligned16(p.weight)) && (reinterpret_cast<uintptr_t>(p.q) & 7) == 0;
+  const int nvec = p.n_cols / E;
+  const dim3 grid((unsigned)n_rows);
+  // the row in registers: at most 8 vectors of 8 values a thread; wider rows are read again instead
+  if (!vec || nvec > 4096) ACACHE_CUDA_CHECK(launch_chained(quantise_any_kernel<T, SRC>, grid, dim3(256), 0, st, p));
+  else if (nvec <= 128) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 128, 1>, grid, dim3(128), 0, st, p));
+  else if (nvec <= 256) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 256, 1>, grid, dim3(256), 0, st, p));
+  else if (nvec <= 512) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 256, 2>, grid, dim3(256), 0, st, p));
+  else if (nvec <= 1024) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 512, 2>, grid, dim3(512), 0, st, p));
+  else if (nvec <= 2048) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 512, 4>, grid, dim3(512), 0, st, p));
+  else ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 512, 8>, grid, dim3(512), 0, st, p));
+  ACACHE_LAUNCH_CHECK();
+  return ACACHE_OK;
+}
+
+}  // namespace quant
+}  // namespace acache
+
+using namespace acache;
+
+extern "C" int acache_quantize_rows(const void* x, int64_t x_stride, int n_rows, int n_cols, int dtype, int8_t* q,
+                                    float* scale, void* stream) {
+  if (!dtype_ok(dtype) || n_rows < 0 || n_cols <= 0) return ACACHE_EINVAL;
+  if (n_rows == 0) return ACACHE_OK;
+  if (!x || !q || !scale) return ACACHE_EINVAL;
+  const quant::Params p{x, x_stride, nullptr, 0, nullptr, 0.f, 0, q, scale, n_cols};
+  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_ROWS>(p, n_rows, (cudaStream_t)stream)));
+  return ACACHE_EINVAL;
+}
+
+extern "C" int acache_rmsnorm_int8(void* x, int64_t x_stride, const void* delta, int64_t d_stride, const void* weight,
+                                   int n_rows, int n_cols, float eps, int dtype, int8_t* q, float* scale, void* stream) {
+  if (!dtype_ok(dtype) || n_rows < 0 || n_cols <= 0) return ACACHE_EINVAL;
+  if (n_rows == 0) return ACACHE_OK;
+  if (!x || !weight || !q || !scale) return ACACHE_EINVAL;
+  const quant::Params p{x, x_stride, delta, d_stride, weight, eps, 0, q, scale, n_cols};
+  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_NORM>(p, n_rows, (cudaStream_t)stream)));
+  return ACACHE_EINVAL;
+}
+
+extern "C" int acache_act_mul_halves_int8(const void* x, int64_t x_stride, int n_rows, int ffn, int act, int dtype,
+                                          int8_t* q, float* scale, void* stream) {
+  if (!dtype_ok(dtype) || n_rows < 0 || ffn <= 0 || act < 0 || act > 2) return ACACHE_EINVAL;
+  if (n_rows == 0) return ACACHE_OK;
+  if (!x || !q || !scale) return ACACHE_EINVAL;
+  const quant::Params p{x, x_stride, nullptr, 0, nullptr, 0.f, act, q, scale, ffn};
+  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_GATE>(p, n_rows, (cudaStream_t)stream)));
+  return ACACHE_EINVAL;
+}

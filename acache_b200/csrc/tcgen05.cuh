@@ -84,6 +84,20 @@ inline bool make_tensor_map_2d(CUtensorMap* map, const void* base, int64_t rows,
          CUDA_SUCCESS;
 }
 
+// the same for a [rows, cols] matrix of bytes: boxes of box_rows x 128 columns
+inline bool make_tensor_map_2d_i8(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t row_stride,
+                                  int box_rows) {
+  EncodeTiledFn fn = tensor_map_encoder();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)row_stride};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // shared-memory matrix descriptor, 128-byte swizzle, atoms of 8 rows x 128 B
 //   lbo/sbo in bytes; K-major operands ignore lbo (set to 16), MN-major use it as the
 //   distance between 64-element column groups
@@ -100,6 +114,11 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t saddr, uint32_t lbo_bytes
 // instruction descriptor: fp32 accumulate, A/B format (0 = f16, 1 = bf16), majors, N, M
 __device__ __forceinline__ uint32_t make_idesc(uint32_t fmt, uint32_t b_mn_major, uint32_t N, uint32_t M) {
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (0u << 15) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+// the same for signed 8-bit integers with 32-bit integer accumulation (kind::i8), both operands K-major
+__device__ __forceinline__ uint32_t make_idesc_i8(uint32_t N, uint32_t M) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
 __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {

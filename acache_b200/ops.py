@@ -1,12 +1,15 @@
 """Operators that replace eager PyTorch sequences of the reference engine:
 anchor scoring and top-k, RoPE + K/V scatter, RMSNorm, gated activation and
-threshold unmasking.  Thin wrappers over the C ABI."""
+threshold unmasking; projections in 8-bit integers and rotary positions from frequencies.
+Thin wrappers over the C ABI."""
 from __future__ import annotations
+
+import math
 
 import torch
 
 from . import _lib
-from ._lib import check, dtype_code, ptr, stream_ptr
+from ._lib import check, dtype_code, on_device_of, ptr, stream_ptr
 
 _ACT = {"silu": 0, "relu": 1, "gelu": 2}
 
@@ -281,6 +284,165 @@ def linear_argmax(x: torch.Tensor, weight: torch.Tensor):
                                        ptr(conf), ptr(scratch), scratch.numel(), GEMM_TILE[0], GEMM_TILE[1],
                                        ptr(_lib.err_flag(x.device)), stream_ptr()), "linear_argmax", 2)
     return x0, conf
+
+
+# ---- projections in 8-bit integers -----------------------------------------------------------
+def _rows_of(x: torch.Tensor):
+    assert x.is_cuda and x.dim() == 2 and x.shape[1] > 0 and x.stride(1) == 1, "rows of a 2-D CUDA tensor, dense inside a row"
+    return x.shape
+
+
+def _int8_rows(x, n, cols):
+    return (torch.empty(n, cols, dtype=torch.int8, device=x.device), torch.empty(n, dtype=torch.float32, device=x.device))
+
+
+def quantize_rows(x: torch.Tensor):
+    """``x [n, cols]`` (fp32 / fp16 / bf16) -> ``(q int8 [n, cols], scale fp32 [n])`` with ``scale = max|x_i| / 127``
+    and ``q = round(127 x / max|x_i|)``, ties to even.  The input of ``linear_int8`` (one scale per token), and its
+    weight (one row per output channel).  A row of zeros has scale 0, a row with an infinity or a NaN scale NaN."""
+    n, cols = _rows_of(x)
+    q, scale = _int8_rows(x, n, cols)
+    if n:
+        with on_device_of(x):
+            check(_lib.load().acache_quantize_rows(ptr(x), x.stride(0), n, cols, dtype_code(x.dtype), ptr(q), ptr(scale),
+                                                   stream_ptr()), "quantize_rows")
+    return q, scale
+
+
+def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: torch.Tensor | None = None):
+    """``quantize_rows`` of ``weight * x * rsqrt(mean(x^2) + eps)`` in one kernel, the norm kept in fp32 up to the
+    rounding.  ``delta`` (optional): a residual update added to ``x`` IN PLACE first, as in ``add_rmsnorm``."""
+    n, cols = _rows_of(x)
+    assert weight.shape == (cols,) and weight.dtype == x.dtype and weight.is_contiguous() and weight.device == x.device
+    if delta is not None:
+        assert delta.shape == x.shape and delta.dtype == x.dtype and delta.stride(1) == 1 and delta.device == x.device
+    q, scale = _int8_rows(x, n, cols)
+    if n:
+        with on_device_of(x):
+            check(_lib.load().acache_rmsnorm_int8(
+                ptr(x), x.stride(0), ptr(delta), delta.stride(0) if delta is not None else 0, ptr(weight), n, cols,
+                float(eps), dtype_code(x.dtype), ptr(q), ptr(scale), stream_ptr()), "rmsnorm_int8")
+    return q, scale
+
+
+def act_mul_halves_int8(x: torch.Tensor, act: str = "silu"):
+    """``quantize_rows`` of ``act(x[:, :F]) * x[:, F:]`` for ``x [n, 2F]`` in one kernel, the product kept in fp32."""
+    n, cols = _rows_of(x)
+    assert cols % 2 == 0
+    q, scale = _int8_rows(x, n, cols // 2)
+    if n:
+        with on_device_of(x):
+            check(_lib.load().acache_act_mul_halves_int8(ptr(x), x.stride(0), n, cols // 2, _ACT[act], dtype_code(x.dtype),
+                                                         ptr(q), ptr(scale), stream_ptr()), "act_mul_halves_int8")
+    return q, scale
+
+
+def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(x int8 [n, in] @ weight int8 [out, in]^T) * x_scale[n, None] * weight_scale[None, out] (+ bias)`` with exact
+    32-bit integer sums, rounded once to ``out_dtype`` (bf16 / fp16).  ``in`` and ``out`` are multiples of 16."""
+    n, k = _rows_of(x)
+    N = weight.shape[0]
+    assert x.dtype == torch.int8 and weight.dtype == torch.int8 and weight.shape == (N, k) and weight.is_contiguous()
+    assert x_scale.shape == (n,) and x_scale.dtype == torch.float32 and x_scale.is_contiguous()
+    assert weight_scale.shape == (N,) and weight_scale.dtype == torch.float32 and weight_scale.is_contiguous()
+    assert weight.device == x.device and x_scale.device == x.device and weight_scale.device == x.device
+    if bias is not None:
+        assert bias.shape == (N,) and bias.dtype == out_dtype and bias.is_contiguous() and bias.device == x.device
+    out = torch.empty(n, N, dtype=out_dtype, device=x.device)
+    if n:
+        with on_device_of(x):
+            check(_lib.load().acache_linear_int8(
+                ptr(x), x.stride(0), ptr(x_scale), n, k, ptr(weight), ptr(weight_scale), N, ptr(bias), dtype_code(out_dtype),
+                ptr(out), out.stride(0), GEMM_TILE[0], GEMM_TILE[1], ptr(_lib.err_flag(x.device)), stream_ptr()),
+                "linear_int8")
+    return out
+
+
+# ---- rotary positions from frequencies -------------------------------------------------------
+def rope_frequencies(rotary_dim: int, theta: float, scaling: dict | None = None, seq_len: int = 0):
+    """``(inv_freq float64 [rotary_dim / 2] on the CPU, attention_factor)`` of a rotary embedding, stretched for
+    contexts beyond the trained one (``original = scaling["original_max_position_embeddings"]``) by
+    ``scaling["rope_type"]``:
+
+    * ``linear``   every frequency divided by ``factor``;
+    * ``ntk``      the base grown so that the slowest pair turns ``factor`` times slower;
+    * ``dynamic``  ``ntk`` with the factor that ``seq_len`` tokens need, no stretch up to ``original``;
+    * ``yarn``     pairs of more than ``beta_fast`` turns over ``original`` kept, of fewer than ``beta_slow``
+      divided by ``factor``, a ramp between; ``attention_factor = 0.1 ln(factor) + 1`` unless given;
+    * ``llama3``   wavelengths below ``original / high_freq_factor`` kept, above ``original / low_freq_factor``
+      divided by ``factor``, a smooth blend between."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim} is not a positive even number")
+    pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "default":
+        return float(theta) ** -pair, 1.0
+    factor = float(scaling["factor"])
+    if factor < 1.0:
+        raise ValueError(f"rope scaling factor {factor} below 1")
+    if kind == "linear":
+        return float(theta) ** -pair / factor, 1.0
+    if kind in ("ntk", "dynamic"):
+        if kind == "dynamic":
+            original = float(scaling["original_max_position_embeddings"])
+            factor = max(factor * seq_len / original - (factor - 1.0), 1.0)
+        grow = factor ** (rotary_dim / (rotary_dim - 2)) if rotary_dim > 2 else factor
+        return (float(theta) * grow) ** -pair, 1.0
+    inv = float(theta) ** -pair
+    original = float(scaling["original_max_position_embeddings"])
+    if kind == "yarn":
+        def dim_of(turns):       # the (fractional) pair index times two that makes `turns` turns over `original`
+            return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        low = max(math.floor(dim_of(float(scaling.get("beta_fast", 32)))), 0)
+        high = min(math.ceil(dim_of(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
+        ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        attention = scaling.get("attention_factor")
+        return inv / factor * ramp + inv * (1 - ramp), float(attention) if attention else 0.1 * math.log(factor) + 1.0
+    if kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        keep = ((original * inv / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        return inv * keep + inv / factor * (1 - keep), 1.0
+    raise ValueError(f"unknown rope_type {kind!r}")
+
+
+def rope_append(q, k, v, positions, inv_freq, k_cache=None, v_cache=None, slot_mapping=None, *, interleaved: bool = False,
+                attention_factor: float = 1.0):
+    """Rotates ``q [n, nh, D]`` and ``k [n, Hkv, D]`` by ``positions`` int64 ``[n]`` times ``inv_freq`` float64
+    ``[rotary_dim / 2]`` (on the device, from ``rope_frequencies``) on the first ``rotary_dim`` dimensions of a head,
+    and appends the rotated ``k`` and ``v`` to the paged caches at ``slot_mapping`` int32 ``[n]`` (-1 skips a row).
+    Returns the rotated queries (a new tensor; ``q`` and ``k`` stay as they are).  Without caches returns the rotated
+    ``(q, k)``.  ``interleaved``: pairs (2j, 2j + 1) instead of (j, j + rotary_dim / 2).  ``attention_factor``
+    multiplies sine and cosine.  The table form of the half layout over the whole head is ``rope_store``."""
+    n, nh, D = q.shape
+    hkv = k.shape[1]
+    assert q.is_cuda and k.shape == (n, hkv, D) and k.dtype == q.dtype and k.device == q.device
+    assert q.stride(2) == 1 and q.stride(1) == D and k.stride(2) == 1 and k.stride(1) == D
+    assert positions.dtype == torch.int64 and positions.shape == (n,) and positions.is_contiguous() and positions.device == q.device
+    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == q.device
+    assert 2 * inv_freq.numel() <= D, "more frequencies than pairs in a head"
+    out_q = torch.empty(n, nh, D, dtype=q.dtype, device=q.device)
+    num_slots, out_k = 0, None
+    if slot_mapping is not None:
+        assert v is not None and v.shape == k.shape and v.dtype == q.dtype and v.device == q.device
+        assert v.stride(2) == 1 and v.stride(1) == D
+        assert slot_mapping.dtype == torch.int32 and slot_mapping.shape == (n,) and slot_mapping.is_contiguous()
+        assert slot_mapping.device == q.device and k_cache.device == q.device and v_cache.device == q.device
+        assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape
+        assert k_cache.dtype == q.dtype and v_cache.dtype == q.dtype and k_cache.shape[-2:] == (hkv, D)
+        num_slots = k_cache.numel() // (hkv * D)
+    else:
+        assert k_cache is None and v_cache is None, "caches without slot_mapping"
+        out_k = torch.empty(n, hkv, D, dtype=q.dtype, device=q.device)
+        v = None
+    if n:
+        with on_device_of(q):
+            check(_lib.load().acache_rope_append(
+                ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0) if v is not None else 0, n, nh, hkv, D,
+                dtype_code(q.dtype), ptr(positions), ptr(inv_freq), 2 * inv_freq.numel(), int(bool(interleaved)),
+                float(attention_factor), ptr(out_q), out_q.stride(0), ptr(k_cache if out_k is None else out_k),
+                ptr(v_cache), ptr(slot_mapping), num_slots, ptr(_lib.err_flag(q.device)), stream_ptr()), "rope_append")
+    return out_q if out_k is None else (out_q, out_k)
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:

@@ -173,6 +173,48 @@ ACACHE_API int acache_linear_argmax(const void* x, int64_t x_stride, int n_rows,
                                     int out_features, int dtype, int64_t* x0, float* confidence, void* scratch,
                                     int64_t scratch_bytes, int tile_mb, int tile_bn, int32_t* err_flag, void* stream);
 
+/* ------------------------------------------------------------------ projections in 8-bit integers
+ * No counterpart in the reference (its projections run in the model's 16-bit type).
+ *
+ * acache_linear_int8: out[i, j] = (sum_k x[i, k] weight[j, k]) * x_scale[i] * w_scale[j] (+ bias[j]), the
+ * sums exact in 32-bit integers, the rest in fp32, rounded once to dtype (fp16 / bf16, the type of out
+ * and bias).  x rows are x_stride bytes apart, weight[out_features, in_features] is dense; in_features and
+ * out_features multiples of 16, 16-byte aligned pointers, x_stride a multiple of 16, out_stride of 8, else
+ * ACACHE_EUNSUPPORTED; in_features above 131071 could overflow the sums: ACACHE_ELIMIT.  tile_mb / tile_bn
+ * (0 = chosen per launch; tile_bn a multiple of 32 in 64..256) as for acache_linear.
+ *
+ * The three quantising producers write q[n_rows, n_cols] dense and one scale per row: scale = a / 127 and
+ * q = round(127 y / a), ties to even, with a the largest |y| of the row.  A row of zeros gets scale 0, a row
+ * that holds an infinity or a NaN gets scale NaN and zeros.  Any width, stride and alignment.
+ *   acache_quantize_rows       y = x                                   (weights: one row per output channel)
+ *   acache_rmsnorm_int8        y = RMSNorm(x) * weight, not rounded to dtype on the way; delta != NULL: x += delta
+ *                              (rounded to dtype, in place) first, as acache_add_rmsnorm does
+ *   acache_act_mul_halves_int8 y = act(gate) * up of x[n_rows, 2 * ffn] = [gate | up], not rounded on the way */
+ACACHE_API int acache_quantize_rows(const void* x, int64_t x_stride, int n_rows, int n_cols, int dtype, int8_t* q,
+                                    float* scale, void* stream);
+ACACHE_API int acache_rmsnorm_int8(void* x, int64_t x_stride, const void* delta, int64_t d_stride, const void* weight,
+                                   int n_rows, int n_cols, float eps, int dtype, int8_t* q, float* scale, void* stream);
+ACACHE_API int acache_act_mul_halves_int8(const void* x, int64_t x_stride, int n_rows, int ffn, int act, int dtype,
+                                          int8_t* q, float* scale, void* stream);
+ACACHE_API int acache_linear_int8(const int8_t* x, int64_t x_stride, const float* x_scale, int n_rows, int in_features,
+                                  const int8_t* weight, const float* w_scale, int out_features, const void* bias, int dtype,
+                                  void* out, int64_t out_stride, int tile_mb, int tile_bn, int32_t* err_flag, void* stream);
+
+/* ------------------------------------------------------------------ rotary positions from frequencies
+ * acache_rope_store's job without tables (no counterpart in the reference): q[n, n_heads, head_dim] and
+ * k[n, n_kv_heads, head_dim] rotated by positions[i] * inv_freq[0 .. rotary_dim / 2) on their first rotary_dim
+ * dimensions, in pairs (j, j + rotary_dim / 2) or, interleaved != 0, (2j, 2j + 1), cosine and sine multiplied
+ * by attention_factor; the other dimensions are copied.  Angles are formed and reduced in 64 bits, the
+ * rotation is in fp32, rounded once.  Rotated queries go to out_q (rows out_q_stride apart).  With
+ * slot_mapping, rotated keys and values go to the caches out_k / out_v at slot_mapping[i] (-1 skips the row's
+ * k and v; any other slot outside [0, num_slots) is skipped and raises err_flag code 1); without it, to row i
+ * of the dense out_k[n, n_kv_heads, head_dim] (and out_v, if v is not NULL).  Outputs may not overlap inputs. */
+ACACHE_API int acache_rope_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                  int64_t v_stride, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int dtype,
+                                  const int64_t* positions, const double* inv_freq, int rotary_dim, int interleaved,
+                                  float attention_factor, void* out_q, int64_t out_q_stride, void* out_k, void* out_v,
+                                  const int32_t* slot_mapping, int64_t num_slots, int32_t* err_flag, void* stream);
+
 /* ------------------------------------------------------------------ anchor top-k
  * Replaces torch.topk + sort + add in anchor selection (nano-vdllm/model_runner.py:833-843;
  * llada/generate_ACache.py:225-262).  scores: fp32 [n_rows, row_stride] (first n_cols of
