@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .._lib import check, dtype_code, ptr, stream_ptr
+from .._lib import check, dtype_code, on_device_of, ptr, stream_ptr
 
 
 # Set by the engine before a forward so that the optional device timers can attribute an
@@ -168,6 +168,74 @@ def acache_attention(q, k_cache, v_cache, cu_seqlens_q, cu_seqlens_k, read_slot_
                     softmax_scale, read_slot_mapping=read_slot_mapping, shared_prefix_len=shared_prefix_len,
                     shared_kv_lens=shared_kv_lens, affix_shifts=affix_shifts, rope_cos=rope_cos, rope_sin=rope_sin,
                     group_shared_span=group_shared_span)
+    return out
+
+
+def pack_keep_mask(keep: torch.Tensor) -> torch.Tensor:
+    """``keep`` bool ``[batch, prefix_len]`` (True = the request reads that prefix key) -> int32 words
+    ``[batch, 2 * ceil(prefix_len / 64)]``, the form ``shared_prefix_attention`` reads: made once where the same
+    mask serves many calls (the holes of a batch are the same in every layer)."""
+    assert keep.is_cuda and keep.dim() == 2 and keep.dtype == torch.bool and (keep.shape[1] <= 1 or keep.stride(1) == 1)
+    batch, n = keep.shape
+    words = torch.empty(batch, 2 * ((n + 63) // 64), dtype=torch.int32, device=keep.device)
+    with on_device_of(keep):
+        check(_lib.load().acache_pack_keep_mask(ptr(keep), keep.stride(0), batch, n, ptr(words), words.shape[1],
+                                                stream_ptr()), "pack_keep_mask")
+    return words
+
+
+def shared_prefix_attention(q, k_cache, v_cache, prefix_slots, cu_seqlens_q, cu_seqlens_k, read_slot_mapping,
+                            softmax_scale=None, *, prefix_keep=None, max_seqlen_q: int | None = None,
+                            max_seqlen_k: int | None = None):
+    """Bidirectional varlen attention of a batch whose requests all read one prefix, the prefix read once for
+    the whole batch: request ``b`` attends to the cache slots ``prefix_slots`` (int32 ``[prefix_len]``) and to its
+    own ``read_slot_mapping[cu_seqlens_k[b]:cu_seqlens_k[b + 1]]``, which does not repeat the prefix.  An entry of -1
+    in either is a key that takes no part.  ``prefix_keep``: prefix keys that a request drops (its anchors replace
+    them), as bool ``[batch, prefix_len]`` or as the words of ``pack_keep_mask``.  Rows of ``q`` behind the last
+    request are left out of the result (undefined there); a request without any key gets zeros.
+
+    ``acache_attention`` reads the prefix once per request, its grouped form once per two requests."""
+    _check_qkv(q, k_cache, v_cache)
+    _require_cuda(prefix_slots, cu_seqlens_q, cu_seqlens_k, read_slot_mapping, prefix_keep)
+    total_q, nh, D = q.shape
+    hkv = k_cache.shape[-2]
+    batch, P = cu_seqlens_q.numel() - 1, prefix_slots.numel()
+    assert k_cache.shape == v_cache.shape and k_cache.shape[-1] == D and nh % hkv == 0
+    for t in (prefix_slots, cu_seqlens_q, cu_seqlens_k, read_slot_mapping):
+        assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.device == q.device
+    assert batch >= 0 and cu_seqlens_k.numel() == batch + 1
+    assert k_cache.device == q.device and v_cache.device == q.device
+    if prefix_keep is not None:
+        if prefix_keep.dtype == torch.bool:
+            assert prefix_keep.shape == (batch, P)
+            prefix_keep = pack_keep_mask(prefix_keep)
+        assert prefix_keep.dtype == torch.int32 and prefix_keep.shape == (batch, 2 * ((P + 63) // 64))
+        assert prefix_keep.is_contiguous() and prefix_keep.device == q.device
+        if P == 0:
+            prefix_keep = None
+    if softmax_scale is None:
+        softmax_scale = D ** -0.5
+    out = torch.empty(total_q, nh, D, dtype=q.dtype, device=q.device)
+    if total_q == 0 or batch == 0:
+        return out
+    if max_seqlen_q is None:
+        max_seqlen_q = _max_len(cu_seqlens_q)
+    if max_seqlen_k is None:
+        max_seqlen_k = _max_len(cu_seqlens_k)
+    lib = _lib.load()
+    with on_device_of(q):
+        # the call's own scratch: two streams, or two captured graphs, never share it
+        nbytes = lib.acache_shared_prefix_attention_scratch_bytes(total_q, nh, hkv, D, batch, int(max_seqlen_q),
+                                                                  int(max_seqlen_k), P)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        with _lib.timed("attention_decode" if ATTENTION_PHASE == "decode" else "attention_refresh", ATTENTION_WORK):
+            check(lib.acache_shared_prefix_attention(
+                ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(k_cache), ptr(v_cache), k_cache.numel() // (hkv * D),
+                total_q, nh, hkv, D, dtype_code(q.dtype), ptr(prefix_slots), P, ptr(prefix_keep),
+                prefix_keep.stride(0) if prefix_keep is not None else 0, ptr(cu_seqlens_q), ptr(cu_seqlens_k), batch,
+                int(max_seqlen_q), int(max_seqlen_k), ptr(read_slot_mapping), read_slot_mapping.numel(),
+                float(softmax_scale), ptr(scratch), nbytes, ptr(_lib.err_flag(q.device)), stream_ptr()),
+                "shared_prefix_attention", 3)
     return out
 
 

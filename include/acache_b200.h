@@ -350,6 +350,36 @@ ACACHE_API int acache_attention_grouped(const void* q, int64_t q_stride, void* o
                              const void* rope_sin, int64_t rope_row_stride, int rope_rows, int rope_dtype,
                              void* scratch, int64_t scratch_bytes, int32_t* err_flag, void* stream);
 
+/* ------------------------------------------------------------------ attention over a prefix shared by the batch
+ * No counterpart in the reference, which reads the shared span once per request.  Bidirectional attention of
+ * ragged queries q[total_q, n_heads, head_dim] (request b: rows [cu_seqlens_q[b], cu_seqlens_q[b + 1])) over
+ *   the prefix: prefix_slots[prefix_len], flat cache slots that every request reads (-1: a hole for all), less
+ *               the keys whose bit in prefix_keep is 0: bit j % 32 of prefix_keep[b * keep_stride + j / 32]
+ *               (NULL = every key; keep_stride even, rows 8-byte aligned; acache_pack_keep_mask makes the words
+ *               from truth values, keep_stride * 32 >= prefix_len);
+ *   its own keys: read_slot_mapping[cu_seqlens_k[b] .. cu_seqlens_k[b + 1]) (-1: a key that takes no part),
+ *               n_slots entries in all; they do NOT include the prefix.
+ * The prefix is multiplied once with the rows of all requests; long key ranges are split.  A request without any
+ * key gets zeros, a row outside every request is left as it was.  Slots outside the cache are skipped and raise
+ * err_flag code 3.  max_seqlen_q / max_seqlen_k: host-known upper bounds of a request's queries and own keys.
+ * 16-bit dtypes, head_dim 64 or 128, 16-byte aligned rows, else ACACHE_EUNSUPPORTED; at most 2047 requests and
+ * 2^23 (query, head of a group) rows, else ACACHE_ELIMIT.  scratch (16-byte aligned, contents irrelevant) holds
+ * acache_shared_prefix_attention_scratch_bytes() of the same sizes and belongs to the call until it has run. */
+ACACHE_API int64_t acache_shared_prefix_attention_scratch_bytes(int total_q, int n_heads, int n_kv_heads, int head_dim,
+                                                                int batch, int max_seqlen_q, int max_seqlen_k,
+                                                                int prefix_len);
+ACACHE_API int acache_shared_prefix_attention(const void* q, int64_t q_stride, void* out, int64_t o_stride,
+                                              const void* k_cache, const void* v_cache, int64_t num_slots, int total_q,
+                                              int n_heads, int n_kv_heads, int head_dim, int dtype,
+                                              const int32_t* prefix_slots, int prefix_len, const int32_t* prefix_keep,
+                                              int64_t keep_stride, const int32_t* cu_seqlens_q,
+                                              const int32_t* cu_seqlens_k, int batch, int max_seqlen_q, int max_seqlen_k,
+                                              const int32_t* read_slot_mapping, int n_slots, float softmax_scale,
+                                              void* scratch, int64_t scratch_bytes, int32_t* err_flag, void* stream);
+/* keep[b * stride + j] != 0 for j < prefix_len -> words[b * words_stride + j / 32], the bits above prefix_len 0 */
+ACACHE_API int acache_pack_keep_mask(const uint8_t* keep, int64_t stride, int batch, int prefix_len, int32_t* words,
+                                     int64_t words_stride, void* stream);
+
 /* ------------------------------------------------------------------ varlen attention, block tables
  * Replaces baseline_ragged_attention and baseline_decode_attention
  * (nano-vdllm/model/acache_attention.py:132-334,525-640): key j of request b lives at
