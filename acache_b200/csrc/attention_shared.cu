@@ -13,11 +13,11 @@
 // the bytes of K and V) goes to rows_kernel below.
 //
 // rows_kernel: a CTA = (KV head, key range, request, 16 or 32 virtual rows), a virtual row being a (query,
-// head-of-the-GQA-group) pair.  Its four warps split the keys in blocks of 16 and share nothing until the end:
-// each gathers its own blocks through the slot map (16-byte cp.async into a ring of its own, three blocks
-// ahead), multiplies with m16n8k16 tensor-core instructions (fp32 accumulators), keeps its own running
-// maximum, sum and O in registers, and the four are merged through shared memory.  No barrier in the loop.
-// 128-row tcgen05 tiles would leave 3/4 of every product empty here and need the whole CTA in step.
+// head-of-the-GQA-group) pair; a warp = (16 rows, one of four key groups).  The groups split the keys in runs of 32
+// and share nothing until the end: each gathers its own blocks of 16 keys through the slot map (16-byte cp.async into a
+// ring of its own, two blocks ahead, the map looked up further ahead still), multiplies with m16n8k16 tensor-core
+// instructions (fp32 accumulators), keeps its own running maximum, sum and O in registers, and the four are merged
+// through shared memory.  128-row tcgen05 tiles would leave 3/4 or more of every product empty here.
 //
 // A key that a request drops still runs through the products with weight 0, and 0 times an infinity or a NaN in
 // its V row is a NaN: the merge looks for NaN in prefix parts under a keep mask and, when it meets one,
@@ -25,6 +25,8 @@
 #include "attention_parts.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
+
+#include <math.h>
 
 namespace acache {
 namespace shared_prefix {
@@ -36,10 +38,9 @@ using tc::ex2;
 using tc::pack2;
 using tc::smem_u32;
 
-constexpr int NW = 4, NT = NW * 32;   // warps of a CTA
+constexpr int NG = 4;                 // key groups of a CTA
 constexpr int KB = 16;                // keys of a block
-constexpr int NS = 3;                 // blocks in flight per warp
-constexpr int kMaxParts = 64;
+constexpr int NS = 3;                 // stages of a group's ring
 
 // how the final result is formed from the prefix parts
 struct Merge {
@@ -120,88 +121,145 @@ __device__ __noinline__ void recompute_prefix(const parts::Args& a, const parts:
   }
 }
 
-// one warp: parts [begin, end) of a row added to (acc, m, l), acc = the sum of weights 2^(score - m) times V
-template <int D>
-__device__ __forceinline__ void merge_parts(const parts::Seg& s, int begin, int end, int64_t row, float* acc, float& m, float& l) {
-  constexpr int E = D / 32;
+// one warp: parts [begin, end) of N rows added to (acc, m, l), acc = the sum of weights 2^(score - m) times V.
+// The loads of the N rows, and of several parts, are in flight together.
+template <int D, int N>
+__device__ __forceinline__ void merge_parts(const parts::Seg& s, int begin, int end, const int64_t (&row)[N], const bool (&live)[N],
+                                            float (&acc)[N][D / 32], float (&m)[N], float (&l)[N]) {
+  constexpr int E = D / 32, U = N == 1 ? 4 : 2;      // parts whose loads are in flight together
   const int lane = threadIdx.x & 31;
   for (int base = begin; base < end; base += 32) {
-    const int n = min(32, end - base);
-    const float lse = lane < n ? s.lse[(int64_t)(base + lane) * s.n_rows + row] : -INFINITY;
-    const float top = fmaxf(m, warp_max(lse));
-    const float f = m == -INFINITY && l == 0.f ? 0.f : ex2(m - top);
-    const float w = lse == -INFINITY ? 0.f : ex2(lse - top);
-    l = l * f + warp_sum(w);
-    m = top;
+    const int cnt = min(32, end - base);
+    float w[N], v[U][N][E];
+    // O of a part without keys was never written: it is loaded with the others and not used
+    auto load = [&](int i) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = f == 0.f ? 0.f : acc[e] * f;
-    for (int i = 0; i < n; ++i) {
-      const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
-      if (wi == 0.f) continue;                  // a part without keys wrote no O
-      const float* o = s.o + ((int64_t)(base + i) * s.n_rows + row) * D + lane * E;
-      if constexpr (E == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(o);
-        acc[0] = fmaf(wi, v.x, acc[0]);
-        acc[1] = fmaf(wi, v.y, acc[1]);
-        acc[2] = fmaf(wi, v.z, acc[2]);
-        acc[3] = fmaf(wi, v.w, acc[3]);
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(o);
-        acc[0] = fmaf(wi, v.x, acc[0]);
-        acc[1] = fmaf(wi, v.y, acc[1]);
-      }
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const float* o = s.o + ((int64_t)(base + min(i + u, cnt - 1)) * s.n_rows + row[n]) * D + lane * E;
+          if constexpr (E == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(o);
+            v[u][n][0] = x.x; v[u][n][1] = x.y; v[u][n][2] = x.z; v[u][n][3] = x.w;
+          } else {
+            const float2 x = *reinterpret_cast<const float2*>(o);
+            v[u][n][0] = x.x; v[u][n][1] = x.y;
+          }
+        }
+    };
+#pragma unroll
+    for (int n = 0; n < N; ++n) w[n] = live[n] && lane < cnt ? s.lse[(int64_t)(base + lane) * s.n_rows + row[n]] : -INFINITY;
+    load(0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float top = fmaxf(m[n], warp_max(w[n]));
+      // a side without keys has the sum 0; one with nothing but NaN scores has a NaN sum, which reaches the result
+      const float f = m[n] == -INFINITY && l[n] == 0.f ? 0.f : ex2(m[n] - top);
+      w[n] = w[n] == -INFINITY ? 0.f : ex2(w[n] - top);
+      l[n] = l[n] * f + warp_sum(w[n]);
+      m[n] = top;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[n][e] = f == 0.f ? 0.f : acc[n][e] * f;
+    }
+    for (int i = 0; i < cnt; i += U) {
+      if (i > 0) load(i);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          float wi = __shfl_sync(0xFFFFFFFFu, w[n], (i + u) & 31);
+          if (i + u >= cnt) wi = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[n][e] = wi == 0.f ? acc[n][e] : fmaf(wi, v[u][n][e], acc[n][e]);
+        }
     }
   }
 }
 
-// one warp: the row's final value from (acc, m, l) of its own keys and the prefix parts
+// the rare way of a row whose merged value holds a NaN under a keep mask: the prefix side again, key by key
+// where it is NaN
 template <typename T, int D>
-__device__ __forceinline__ void finish_row(const parts::Args& a, const parts::Seg& prefix, const Merge& mg, int q_row, int head,
-                                           float* acc, float m, float l) {
+__device__ __noinline__ void finish_again(const parts::Args& a, const parts::Seg& s, const parts::Seg& prefix, const Merge& mg,
+                                          int own_begin, int own_end, int q_row, int head, const float* own_acc, float own_m,
+                                          float own_l, float* v) {
+  constexpr int E = D / 32;
+  const int64_t row[1] = {(int64_t)q_row * a.n_heads + head};
+  const bool live[1] = {true};
+  float own[1][E], m[1] = {own_m}, l[1] = {own_l}, pre[1][E], pm[1] = {-INFINITY}, pl[1] = {0.f};
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    own[0][e] = own_acc[e];
+    pre[0][e] = 0.f;
+  }
+  merge_parts<D, 1>(s, own_begin, own_end, row, live, own, m, l);
+  merge_parts<D, 1>(s, 0, mg.n_parts, row, live, pre, pm, pl);
+  if (pl[0] > 0.f) {
+    float again[E];
+    recompute_prefix<T, D>(a, prefix, mg, q_row, head, pm[0] + log2f(pl[0]), again);
+#pragma unroll
+    for (int e = 0; e < E; ++e) pre[0][e] = isnan(pre[0][e]) ? again[e] * pl[0] : pre[0][e];
+  }
+  const float top = fmaxf(m[0], pm[0]);
+  const float fo = m[0] == -INFINITY && l[0] == 0.f ? 0.f : ex2(m[0] - top);
+  const float fp = pm[0] == -INFINITY && pl[0] == 0.f ? 0.f : ex2(pm[0] - top);
+  const float inv = 1.f / (l[0] * fo + pl[0] * fp);
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = ((fo == 0.f ? 0.f : own[0][e] * fo) + (fp == 0.f ? 0.f : pre[0][e] * fp)) * inv;
+}
+
+// one warp: the final values of N rows from (acc, m, l) of the keys that have no part in the workspace, the prefix
+// parts and own parts [own_begin, own_end)
+template <typename T, int D, int N>
+__device__ __forceinline__ void finish_rows(const parts::Args& a, const parts::Seg& s, const parts::Seg& prefix, const Merge& mg,
+                                            int own_begin, int own_end, const int (&q_row)[N], const int (&head)[N],
+                                            const bool (&live)[N], float (&acc)[N][D / 32], float (&m)[N], float (&l)[N]) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)q_row * a.n_heads + head;
-  float pre[E], pm = -INFINITY, pl = 0.f;
+  int64_t row[N];
+  float acc0[N][E], m0[N], l0[N];
 #pragma unroll
-  for (int e = 0; e < E; ++e) pre[e] = 0.f;
-  merge_parts<D>(prefix, 0, mg.n_parts, row, pre, pm, pl);
-  if (prefix.keep) {
+  for (int n = 0; n < N; ++n) {
+    row[n] = (int64_t)q_row[n] * a.n_heads + head[n];
+    m0[n] = m[n];
+    l0[n] = l[n];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc0[n][e] = acc[n][e];
+  }
+  // the prefix's parts and the own ones follow each other in the workspace
+  merge_parts<D, N>(s, mg.n_parts > 0 ? 0 : own_begin, mg.n_parts > 0 && own_end == own_begin ? mg.n_parts : own_end, row, live, acc, m, l);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (!live[n]) continue;
+    const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];          // no key at all: zeros
+    float v[E];
     bool bad = false;
 #pragma unroll
-    for (int e = 0; e < E; ++e) bad |= isnan(pre[e]);
-    if (__any_sync(0xFFFFFFFFu, bad) && pl > 0.f) {
-      float again[E];
-      recompute_prefix<T, D>(a, prefix, mg, q_row, head, pm + log2f(pl), again);
-#pragma unroll
-      for (int e = 0; e < E; ++e) pre[e] = isnan(pre[e]) ? again[e] * pl : pre[e];
+    for (int e = 0; e < E; ++e) {
+      v[e] = acc[n][e] * inv;
+      bad |= isnan(v[e]);
     }
+    if (prefix.keep && mg.n_parts > 0 && __any_sync(0xFFFFFFFFu, bad))
+      finish_again<T, D>(a, s, prefix, mg, own_begin, own_end, q_row[n], head[n], acc0[n], m0[n], l0[n], v);
+    T* dst = (T*)mg.out + (int64_t)q_row[n] * mg.o_stride + (int64_t)head[n] * D + lane * E;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    else *reinterpret_cast<uint32_t*>(dst) = pack2<T>(v[0], v[1]);
   }
-  const float top = fmaxf(m, pm);
-  // a side without keys has the sum 0; one with NaN scores has a NaN sum, which reaches the result
-  const float fo = m == -INFINITY && l == 0.f ? 0.f : ex2(m - top), fp = pm == -INFINITY && pl == 0.f ? 0.f : ex2(pm - top);
-  const float total = l * fo + pl * fp;
-  const float inv = total == 0.f ? 0.f : 1.f / total;         // no key at all: zeros
-  float v[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = ((fo == 0.f ? 0.f : acc[e] * fo) + (fp == 0.f ? 0.f : pre[e] * fp)) * inv;
-  T* dst = (T*)mg.out + (int64_t)q_row * mg.o_stride + (int64_t)head * D + lane * E;
-  if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-  else *reinterpret_cast<uint32_t*>(dst) = pack2<T>(v[0], v[1]);
 }
 
 // FINAL: the segment is the requests' own keys in one range each: the CTA also merges the prefix parts (written by
 // the kernel before it in the stream, beside which it may run) and writes the output.  Else it leaves a part.
-template <typename T, int D, int MT, bool FINAL>
-__global__ void __launch_bounds__(NT, 2) rows_kernel(const __grid_constant__ parts::Args a, const __grid_constant__ parts::Seg s,
-                                                     const __grid_constant__ parts::Seg prefix, const __grid_constant__ Merge mg,
-                                                     int beside) {
-  constexpr int ROWS = MT * 16, CH = D / 8, KS = D / 16, E = D / 32;
+template <typename T, int D, int RT, bool FINAL>
+__global__ void __launch_bounds__(RT * NG * 32, 2) rows_kernel(const __grid_constant__ parts::Args a, const __grid_constant__ parts::Seg s,
+                                                               const __grid_constant__ parts::Seg prefix,
+                                                               const __grid_constant__ Merge mg, int beside) {
+  constexpr int NT = RT * NG * 32, ROWS = RT * 16, CH = D / 8, KS = D / 16, E = D / 32;
   constexpr int BLOCK = KB * D * 2;             // bytes of K (or V) of a block
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* sQ = smem;                           // [ROWS][D]
-  uint8_t* ring = smem + ROWS * D * 2;          // [NW][NS][K | V]
-  __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
+  uint8_t* ring = smem + ROWS * D * 2;          // [NG][NS][K | V]
+  __shared__ float s_m[NG][ROWS], s_l[NG][ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int grp = warp % NG, rt = warp / NG;    // key group and row tile of the warp
 
   // beside: the kernel before this one in the stream belongs to the same call and this one reads nothing
   // of it before the merge; the kernels before that one have completed
@@ -210,13 +268,27 @@ __global__ void __launch_bounds__(NT, 2) rows_kernel(const __grid_constant__ par
   const int g = a.n_heads / a.n_kv_heads, kvh = blockIdx.x, b = blockIdx.z;
   const int split = blockIdx.y % s.splits, m0 = blockIdx.y / s.splits * ROWS;
   parts::Range r = parts::request_range(s, b);
-  const int first_key = parts::split_range(s, split, KB * NW, r);
+  const int first_key = parts::split_range(s, split, 2 * KB * NG, r);
   const int vrows = r.n_q * g;
   if (m0 >= vrows) {
     if (beside) chain_wait();                   // this grid may not end before the one it runs beside
     return;
   }
   const int64_t kv_row = (int64_t)a.n_kv_heads * D;
+
+  // ---- the keys of this group: runs of 32 (two blocks) grp, grp + NG, ...; one load looks a run's slots up,
+  // three runs ahead of their use
+  const int n_runs = (r.n_k + 2 * KB - 1) / (2 * KB), my_runs = n_runs > grp ? (n_runs - grp + NG - 1) / NG : 0;
+  const int mine = 2 * my_runs;                 // blocks; the last may lie behind the end
+  const uint32_t my_ring = smem_u32(ring) + grp * (NS * 2 * BLOCK);
+  const T* kc = (const T*)a.k_cache + (int64_t)kvh * D;
+  const T* vc = (const T*)a.v_cache + (int64_t)kvh * D;
+  // lane l holds the slot of key l of a run; -1 = takes no part
+  auto slots_of = [&](int u) -> int32_t {
+    const int j = (grp + u * NG) * 2 * KB + lane;
+    return u < my_runs && j < r.n_k ? s.slots[r.k0 + j] : -1;
+  };
+  int32_t run_now = slots_of(0), run_a = slots_of(1), run_b = slots_of(2);
 
   // ---- queries
   for (int i = tid; i < ROWS * CH; i += NT) {
@@ -227,173 +299,131 @@ __global__ void __launch_bounds__(NT, 2) rows_kernel(const __grid_constant__ par
   }
   cp_async_commit();
 
-  // ---- the keys of this warp: blocks warp, warp + NW, ...
-  const int n_blocks = (r.n_k + KB - 1) / KB;
-  const int mine = n_blocks > warp ? (n_blocks - warp + NW - 1) / NW : 0;
-  const uint32_t my_ring = smem_u32(ring) + warp * (NS * 2 * BLOCK);
-  const T* kc = (const T*)a.k_cache + (int64_t)kvh * D;
-  const T* vc = (const T*)a.v_cache + (int64_t)kvh * D;
-  // lane l (and l + 16) holds the slot of key l of a block; -1 = takes no part
-  auto slot_of = [&](int i) -> int32_t {
-    const int j = (warp + i * NW) * KB + (lane & 15);
-    return i < mine && j < r.n_k ? s.slots[r.k0 + j] : -1;
-  };
-  auto check_slot = [&](int32_t v) -> int32_t {
-    if (v < -1 || v >= a.num_slots) {
-      if (a.err_flag) atomicExch(a.err_flag, 3);
-      return -1;
-    }
-    return v;
-  };
-  auto gather = [&](int i, int32_t slot) {      // block i into its stage
+  auto gather = [&](int i) -> uint32_t {        // block i into its stage (each row tile's warp a part of it); its dead keys
     const uint32_t kb = my_ring + (i % NS) * (2 * BLOCK), vb = kb + BLOCK;
-    constexpr int RPI = 32 / CH;                // rows per step of the warp
-    const int c = lane % CH;
-#pragma unroll
-    for (int it = 0; it < KB / RPI; ++it) {
-      const int row = it * RPI + lane / CH;
-      const int32_t sl = __shfl_sync(0xFFFFFFFFu, slot, row);
-      const int64_t off = (int64_t)(sl < 0 ? 0 : sl) * kv_row + c * 8;
-      cp_async16(kb + at<D>(row, c), kc + off, sl >= 0);
-      cp_async16(vb + at<D>(row, c), vc + off, sl >= 0);
+    constexpr int RPI = 32 / CH, STEPS = KB / RPI / RT;     // rows per step of the warp
+    const int c = lane % CH, half = (i & 1) * KB;
+    int32_t slot = run_now;
+    if (slot < -1 || slot >= a.num_slots) {
+      if (a.err_flag) atomicExch(a.err_flag, 3);
+      slot = -1;
     }
+    const uint32_t dead = __ballot_sync(0xFFFFFFFFu, slot < 0) >> half;
+    if (i < mine) {
+#pragma unroll
+      for (int it = 0; it < STEPS; ++it) {
+        const int row = (rt * STEPS + it) * RPI + lane / CH;
+        const int32_t sl = __shfl_sync(0xFFFFFFFFu, slot, half + row);
+        const int64_t off = (int64_t)(sl < 0 ? 0 : sl) * kv_row + c * 8;
+        cp_async16(kb + at<D>(row, c), kc + off, sl >= 0);
+        cp_async16(vb + at<D>(row, c), vc + off, sl >= 0);
+      }
+    }
+    cp_async_commit();
+    if (i & 1) {
+      run_now = run_a;
+      run_a = run_b;
+      run_b = slots_of(i / 2 + 3);
+    }
+    return dead;
+  };
+  // the warps that share a group's blocks
+  auto group_sync = [&]() {
+    if constexpr (RT == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(RT * 32) : "memory");
   };
   // dead keys of the blocks in flight, oldest first
   uint32_t dead_q[NS];
-  int32_t next_slot = slot_of(0);
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) {
-    const int32_t slot = check_slot(next_slot);
-    next_slot = slot_of(i + 1);
-    dead_q[i] = __ballot_sync(0xFFFFFFFFu, slot < 0);
-    if (i < mine) gather(i, slot);
-    cp_async_commit();
-  }
+  for (int i = 0; i < NS - 1; ++i) dead_q[i] = gather(i);
 
-  // which keys the rows of this thread keep: rows lane / 4 + 8 h
-  const uint16_t* keep[2 * MT];
+  // which keys the rows of this thread keep: rows lane / 4 + 8 h of the tile
+  const uint16_t* keep[2];
   if (s.keep) {
 #pragma unroll
-    for (int h = 0; h < 2 * MT; ++h) {
-      const int vr = min(m0 + lane / 4 + 8 * h, vrows - 1);
+    for (int h = 0; h < 2; ++h) {
+      const int vr = min(m0 + rt * 16 + lane / 4 + 8 * h, vrows - 1);
       keep[h] = reinterpret_cast<const uint16_t*>(s.keep + (int64_t)parts::request_of(s.req_cu, s.n_req, r.q0 + vr / g) * s.keep_stride) + first_key / KB;
     }
   }
-
   cp_async_wait<NS - 1>();
   __syncthreads();                              // the queries have landed
-  uint32_t qa[MT == 1 ? KS : 1][4];
   const uint32_t q_addr = smem_u32(sQ);
-  if constexpr (MT == 1) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ldsm4(q_addr + at<D>(lane & 15, 2 * ks + (lane >> 4)), qa[ks]);
-  }
 
-  float o[MT][D / 8][4], m_ref[2 * MT], l_sum[2 * MT];
+  float o[D / 8][4], m_ref[2] = {-INFINITY, -INFINITY}, l_sum[2] = {0.f, 0.f};
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+  for (int d = 0; d < D / 8; ++d)
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[t][d][e] = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2 * MT; ++h) {
-    m_ref[h] = -INFINITY;
-    l_sum[h] = 0.f;
-  }
+    for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
 
   for (int i = 0; i < mine; ++i) {
-    {
-      const int32_t slot = check_slot(next_slot);
-      next_slot = slot_of(i + NS);
-      dead_q[NS - 1] = __ballot_sync(0xFFFFFFFFu, slot < 0);
-      if (i + NS - 1 < mine) gather(i + NS - 1, slot);
-      cp_async_commit();
-    }
-    uint32_t kept[2 * MT];
+    uint32_t kept[2];
     if (s.keep) {
 #pragma unroll
-      for (int h = 0; h < 2 * MT; ++h) kept[h] = keep[h][warp + i * NW];
+      for (int h = 0; h < 2; ++h) kept[h] = keep[h][2 * (grp + (i / 2) * NG) + (i & 1)];
     }
-    cp_async_wait<NS - 1>();
-    __syncwarp();
+    cp_async_wait<NS - 2>();
+    group_sync();                               // block i is there, block i - 1 has been read by all
+    dead_q[NS - 1] = gather(i + NS - 1);
     const uint32_t kb = my_ring + (i % NS) * (2 * BLOCK), vb = kb + BLOCK;
 
-    // ---- scores: keys 0-7 and 8-15 of the block against every row tile
-    float sc[MT][2][4];
+    // ---- scores: keys 0-7 and 8-15 of the block against the row tile
+    float sc[2][4];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sc[t][e / 4][e % 4] = 0.f;
+    for (int e = 0; e < 8; ++e) sc[e / 4][e % 4] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      uint32_t kf[4];
+      uint32_t kf[4], qf[4];
       ldsm4(kb + at<D>((lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)), kf);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if constexpr (MT == 1) {
-          mma16816<T>(sc[t][0], qa[ks], kf[0], kf[1]);
-          mma16816<T>(sc[t][1], qa[ks], kf[2], kf[3]);
-        } else {
-          uint32_t qf[4];
-          ldsm4(q_addr + at<D>(t * 16 + (lane & 15), 2 * ks + (lane >> 4)), qf);
-          mma16816<T>(sc[t][0], qf, kf[0], kf[1]);
-          mma16816<T>(sc[t][1], qf, kf[2], kf[3]);
-        }
-      }
+      ldsm4(q_addr + at<D>(rt * 16 + (lane & 15), 2 * ks + (lane >> 4)), qf);
+      mma16816<T>(sc[0], qf, kf[0], kf[1]);
+      mma16816<T>(sc[1], qf, kf[2], kf[3]);
     }
     // ---- keys that take no part, per row under a keep mask
     const uint32_t dead = dead_q[0] & 0xFFFFu;
     if (dead != 0u || s.keep) {
 #pragma unroll
-      for (int h = 0; h < 2 * MT; ++h) {
+      for (int h = 0; h < 2; ++h) {
         const uint32_t gone = (s.keep ? dead | ~kept[h] : dead) >> (2 * (lane & 3));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if ((gone >> ((e & 1) + 8 * (e >> 1))) & 1u) sc[h / 2][e >> 1][2 * (h & 1) + (e & 1)] = -INFINITY;
+          if ((gone >> ((e & 1) + 8 * (e >> 1))) & 1u) sc[e >> 1][2 * h + (e & 1)] = -INFINITY;
       }
     }
 #pragma unroll
     for (int k = 0; k < NS - 1; ++k) dead_q[k] = dead_q[k + 1];
     // ---- online softmax; O is rescaled only when a row's maximum grows by more than 2^8
-    float mx[2 * MT];
-    bool grows = false;
+    float mx[2];
 #pragma unroll
-    for (int h = 0; h < 2 * MT; ++h) {
-      const float* c0 = &sc[h / 2][0][2 * (h & 1)];
-      const float* c1 = &sc[h / 2][1][2 * (h & 1)];
-      float v = fmaxf(fmaxf(c0[0], c0[1]), fmaxf(c1[0], c1[1]));
+    for (int h = 0; h < 2; ++h) {
+      float v = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
       v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
       v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
       mx[h] = v * a.scale_log2;
-      grows |= mx[h] > m_ref[h] + 8.f;
     }
-    if (__any_sync(0xFFFFFFFFu, grows)) {
+    if (__any_sync(0xFFFFFFFFu, mx[0] > m_ref[0] + 8.f || mx[1] > m_ref[1] + 8.f)) {
 #pragma unroll
-      for (int h = 0; h < 2 * MT; ++h) {
+      for (int h = 0; h < 2; ++h) {
         const bool grow = mx[h] > m_ref[h] + 8.f;
         const float f = grow ? ex2(m_ref[h] - mx[h]) : 1.f;
         if (grow) m_ref[h] = mx[h];
         l_sum[h] *= f;
 #pragma unroll
         for (int d = 0; d < D / 8; ++d) {
-          o[h / 2][d][2 * (h & 1)] *= f;
-          o[h / 2][d][2 * (h & 1) + 1] *= f;
+          o[d][2 * h] *= f;
+          o[d][2 * h + 1] *= f;
         }
       }
     }
-    uint32_t pa[MT][4];
+    uint32_t pa[4];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int h = 0; h < 2; ++h) {
+      const float mu = m_ref[h] == -INFINITY ? 0.f : m_ref[h];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float mu = m_ref[2 * t + h] == -INFINITY ? 0.f : m_ref[2 * t + h];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float p0 = ex2(fmaf(sc[t][n][2 * h], a.scale_log2, -mu)), p1 = ex2(fmaf(sc[t][n][2 * h + 1], a.scale_log2, -mu));
-          l_sum[2 * t + h] += p0 + p1;
-          pa[t][2 * n + h] = pack2<T>(p0, p1);
-        }
+      for (int n = 0; n < 2; ++n) {
+        const float p0 = ex2(fmaf(sc[n][2 * h], a.scale_log2, -mu)), p1 = ex2(fmaf(sc[n][2 * h + 1], a.scale_log2, -mu));
+        l_sum[h] += p0 + p1;
+        pa[2 * n + h] = pack2<T>(p0, p1);
       }
     }
     // ---- O += P V
@@ -401,83 +431,101 @@ __global__ void __launch_bounds__(NT, 2) rows_kernel(const __grid_constant__ par
     for (int d = 0; d < D / 16; ++d) {
       uint32_t vf[4];
       ldsm4t(vb + at<D>(lane & 15, 2 * d + (lane >> 4)), vf);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        mma16816<T>(o[t][2 * d], pa[t], vf[0], vf[1]);
-        mma16816<T>(o[t][2 * d + 1], pa[t], vf[2], vf[3]);
-      }
+      mma16816<T>(o[2 * d], pa, vf[0], vf[1]);
+      mma16816<T>(o[2 * d + 1], pa, vf[2], vf[3]);
     }
-    __syncwarp();                               // the stage may be written again
   }
   cp_async_wait<0>();
 
-  // ---- the four warps' results through shared memory (over the ring)
+  // ---- the groups' results through shared memory (over the ring)
   __syncthreads();
-  constexpr int LD = D + 4;
-  float* sO = reinterpret_cast<float*>(ring);   // [NW][ROWS][LD]
+  constexpr int LD = D + 8;                     // rows 8 banks apart: the float2 stores of a half warp do not collide
+  float* sO = reinterpret_cast<float*>(ring);   // [NG][ROWS][LD]
 #pragma unroll
-  for (int h = 0; h < 2 * MT; ++h) {
-    const int row = lane / 4 + 8 * h;
+  for (int h = 0; h < 2; ++h) {
+    const int row = rt * 16 + lane / 4 + 8 * h;
     float l = l_sum[h];
     l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
     l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
     if ((lane & 3) == 0) {
-      s_m[warp][row] = m_ref[h];
-      s_l[warp][row] = l;
+      s_m[grp][row] = m_ref[h];
+      s_l[grp][row] = l;
     }
 #pragma unroll
     for (int d = 0; d < D / 8; ++d)
-      *reinterpret_cast<float2*>(sO + (warp * ROWS + row) * LD + d * 8 + 2 * (lane & 3)) =
-          make_float2(o[h / 2][d][2 * (h & 1)], o[h / 2][d][2 * (h & 1) + 1]);
+      *reinterpret_cast<float2*>(sO + (grp * ROWS + row) * LD + d * 8 + 2 * (lane & 3)) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
   }
   __syncthreads();
   if (beside) chain_wait();                     // the prefix parts are there
-  for (int row = warp; row < ROWS && m0 + row < vrows; row += NW) {
-    float m = -INFINITY, l = 0.f, acc[E];
+  constexpr int N = 4;                          // rows of a warp: warp, warp + NW, ...
+  float acc[N][E], m[N], l[N];
+  int q_row[N], head[N];
+  bool live[N];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, s_m[w][row]);
+  for (int n = 0; n < N; ++n) {
+    const int row = warp + n * (RT * NG), vr = m0 + row;
+    live[n] = vr < vrows;
+    q_row[n] = r.q0 + (live[n] ? vr / g : 0);
+    head[n] = kvh * g + (live[n] ? vr % g : 0);
+    m[n] = -INFINITY;
+    l[n] = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int w = 0; w < NG; ++w) m[n] = fmaxf(m[n], s_m[w][row]);
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = s_m[w][row];
-      if (mw == -INFINITY && s_l[w][row] == 0.f) continue;   // no key (only NaN scores leave a NaN sum)
-      const float f = ex2(mw - m);
-      l = fmaf(f, s_l[w][row], l);
+    for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, sO[(w * ROWS + row) * LD + lane * E + e], acc[e]);
-    }
-    const int vr = m0 + row, q_row = r.q0 + vr / g, head = kvh * g + vr % g;
-    if constexpr (FINAL) {
-      finish_row<T, D>(a, prefix, mg, q_row, head, acc, m, l);
-    } else {
-      const int64_t at_row = (int64_t)(s.first_part + split) * s.n_rows + (int64_t)q_row * a.n_heads + head;
-      const bool any_key = m != -INFINITY || l != 0.f;
-      if (any_key) {
-        const float inv = 1.f / l;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s.o[at_row * D + lane * E + e] = acc[e] * inv;
+    for (int w = 0; w < NG; ++w) {
+      const float mw = s_m[w][row], lw = s_l[w][row];
+      const bool none = mw == -INFINITY && lw == 0.f;        // no key (only NaN scores leave a NaN sum)
+      const float f = none ? 0.f : ex2(mw - m[n]);
+      l[n] = fmaf(f, lw, l[n]);
+      float x[E];
+      const float* src = sO + (w * ROWS + row) * LD + lane * E;
+      if constexpr (E == 4) {
+        const float4 t = *reinterpret_cast<const float4*>(src);
+        x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+      } else {
+        const float2 t = *reinterpret_cast<const float2*>(src);
+        x[0] = t.x; x[1] = t.y;
       }
-      if (lane == 0) s.lse[at_row] = any_key ? m + log2f(l) : -INFINITY;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[n][e] = none ? acc[n][e] : fmaf(f, x[e], acc[n][e]);
+    }
+  }
+  if constexpr (FINAL) {
+    finish_rows<T, D, N>(a, s, prefix, mg, s.first_part, s.first_part, q_row, head, live, acc, m, l);
+  } else {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (!live[n]) continue;
+      const int64_t at_row = (int64_t)(s.first_part + split) * s.n_rows + (int64_t)q_row[n] * a.n_heads + head[n];
+      const bool any_key = m[n] != -INFINITY || l[n] != 0.f;
+      if (any_key) {
+        const float inv = 1.f / l[n];
+        float* dst = s.o + at_row * D + lane * E;
+        if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc[n][0] * inv, acc[n][1] * inv, acc[n][2] * inv, acc[n][3] * inv);
+        else *reinterpret_cast<float2*>(dst) = make_float2(acc[n][0] * inv, acc[n][1] * inv);
+      }
+      if (lane == 0) s.lse[at_row] = any_key ? m[n] + log2f(l[n]) : -INFINITY;
     }
   }
 }
 
-// one warp per row: own parts and prefix parts into the output
+// one warp per row: prefix parts and own parts into the output
 template <typename T, int D>
 __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ parts::Args a, const __grid_constant__ parts::Seg own,
                                                     const __grid_constant__ parts::Seg prefix, const __grid_constant__ Merge mg, int n_req) {
   chain_release();
   chain_wait();
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int q_row = (int)(row / a.n_heads), head = (int)(row % a.n_heads);
+  const int q_row[1] = {(int)(row / a.n_heads)}, head[1] = {(int)(row % a.n_heads)};
   // rows behind the last sequence (or before the first) have no result
-  if (q_row >= own.total_q || q_row < own.cu_q[0] || q_row >= own.cu_q[n_req]) return;
-  float acc[D / 32], m = -INFINITY, l = 0.f;
+  if (q_row[0] >= own.total_q || q_row[0] < own.cu_q[0] || q_row[0] >= own.cu_q[n_req]) return;
+  const bool live[1] = {true};
+  float acc[1][D / 32], m[1] = {-INFINITY}, l[1] = {0.f};
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-  merge_parts<D>(own, own.first_part, own.first_part + own.splits, row, acc, m, l);
-  finish_row<T, D>(a, prefix, mg, q_row, head, acc, m, l);
+  for (int e = 0; e < D / 32; ++e) acc[0][e] = 0.f;
+  finish_rows<T, D, 1>(a, own, prefix, mg, own.first_part, own.first_part + own.splits, q_row, head, live, acc, m, l);
 }
 
 // 32 truth values to a word: bit j of word w of a row is key 32 w + j
@@ -498,37 +546,62 @@ struct Plan {
   int prefix_splits, own_splits;
 };
 
-static int clamp_splits(int64_t want, int64_t keys, int min_keys) {
-  const int64_t most = keys / min_keys;
-  if (want > most) want = most;
-  if (want > 32) want = 32;
-  return want < 1 ? 1 : (int)want;
+// What a segment costs.  Measured on B200 (bf16, head_dim 128): 64 keys take a 256-row CTA 1.45 us (one CTA per SM) and
+// its start and end about 8 us; 64 keys take a rows_kernel CTA about 1.2 us (two per SM) and its start and end 7 us;
+// partial results are fp32, written and read back at about 4 TB/s.
+struct Cost {
+  double tile, fixed;                 // us
+  int per_sm;
+  int64_t units, tiles;               // CTAs in one range each, 64-key tiles of the longest request
+  double cta(int s) const { return fixed + tile * ((tiles + s - 1) / s); }
+  double latency(int s) const { return cta(s) * ((units * s + kNumSMs * per_sm - 1) / (kNumSMs * per_sm)); }
+  double sm_time(int s) const { return cta(s) * units * s / per_sm; }
+};
+static Cost cost_of(bool wide, int64_t requests, int64_t rows_per_request, int64_t keys, int n_kv_heads) {
+  const int64_t tile_rows = wide ? 256 : (rows_per_request <= 16 ? 16 : 32);
+  Cost c{wide ? 1.45 : 1.2, wide ? 8.0 : 7.0, wide ? 1 : 2, n_kv_heads * requests * ((rows_per_request + tile_rows - 1) / tile_rows),
+         (keys + 63) / 64};
+  return c;
 }
 
-static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_len, int n_heads, int n_kv_heads) {
+// The two segments run beside each other: the ranges per request are chosen so that the longer of them, and the sum of
+// their work over all SMs, take the least time together with the traffic of the partial results.
+static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_len, int n_heads, int n_kv_heads, int head_dim) {
   const int64_t g = n_heads / n_kv_heads, all = total_q * g, per_request = max_q * g;
+  const double part_us = (double)total_q * n_heads * head_dim * 8 / 4.0e6;
   Plan p;
   p.prefix_wide = all > 32;
   p.own_wide = per_request > 128;
-  if (p.prefix_wide) p.prefix_splits = clamp_splits(kNumSMs / (n_kv_heads * ((all + 255) / 256)), prefix_len, 256);
-  else p.prefix_splits = clamp_splits(2 * kNumSMs / (n_kv_heads * ((all + 31) / 32)), prefix_len, 128);
-  if (p.own_wide) p.own_splits = clamp_splits(kNumSMs / (n_kv_heads * batch * ((per_request + 255) / 256)), max_k, 256);
-  else p.own_splits = clamp_splits(2 * kNumSMs / (n_kv_heads * (int64_t)batch * ((per_request + 31) / 32)), max_k, 256);
+  const Cost pre = cost_of(p.prefix_wide, 1, all, prefix_len, n_kv_heads), own = cost_of(p.own_wide, batch, per_request, max_k, n_kv_heads);
+  double best = 1e30;
+  p.prefix_splits = p.own_splits = 1;
+  for (int so = 1; so <= 32 && (so == 1 || own.tiles / so >= 2); ++so) {
+    for (int sp = 1; sp <= 32 && (sp == 1 || pre.tiles / sp >= 2); ++sp) {
+      const double both = (pre.sm_time(sp) + own.sm_time(so)) / kNumSMs;
+      double t = fmax(both, fmax(pre.latency(sp), own.latency(so))) + (sp + so) * part_us;
+      if (so > 1 || p.own_wide) t += 4.0;          // the merge kernel
+      if (t < best * 0.98) {                       // a few per cent do not pay for more parts
+        best = t;
+        p.prefix_splits = sp;
+        p.own_splits = so;
+      }
+    }
+  }
   return p;
 }
 
-template <typename T, int D, int MT, bool FINAL>
+template <typename T, int D, int RT, bool FINAL>
 static int launch_rows(const parts::Args& a, const parts::Seg& s, const parts::Seg& prefix, const Merge& mg, int n_requests,
                        int max_q, int beside) {
-  constexpr size_t ring = (size_t)NW * NS * 2 * KB * D * 2, merge = (size_t)NW * MT * 16 * (D + 4) * 4;
-  constexpr size_t smem = MT * 16 * D * 2 + (ring > merge ? ring : merge);
-  auto kern = rows_kernel<T, D, MT, FINAL>;
+  constexpr size_t ring = (size_t)NG * NS * 2 * KB * D * 2, merge = (size_t)NG * RT * 16 * (D + 8) * 4;
+  constexpr size_t smem = RT * 16 * D * 2 + (ring > merge ? ring : merge);
+  auto kern = rows_kernel<T, D, RT, FINAL>;
   ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const int g = a.n_heads / a.n_kv_heads;
-  const int64_t tiles = ((int64_t)max_q * g + MT * 16 - 1) / (MT * 16);
+  const int64_t tiles = ((int64_t)max_q * g + RT * 16 - 1) / (RT * 16);
   if (tiles * s.splits > 65535) return ACACHE_ELIMIT;
-  ACACHE_CUDA_CHECK(launch_chained(kern, dim3(a.n_kv_heads, (unsigned)(tiles * s.splits), n_requests), dim3(NT), smem, a.st, a, s,
-                                   prefix, mg, beside));
+  ACACHE_CUDA_CHECK(launch_chained(kern, dim3(a.n_kv_heads, (unsigned)(tiles * s.splits), n_requests), dim3(RT * NG * 32), smem, a.st,
+                                   a, s, prefix, mg, beside));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;
 }
@@ -567,7 +640,7 @@ extern "C" int64_t acache_shared_prefix_attention_scratch_bytes(int total_q, int
   if (total_q <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || batch <= 0 || max_seqlen_q < 0 ||
       max_seqlen_k < 0 || prefix_len < 0)
     return 0;
-  const shared_prefix::Plan p = shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads);
+  const shared_prefix::Plan p = shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads, head_dim);
   const int64_t parts = p.prefix_splits + p.own_splits;
   return parts * total_q * n_heads * (int64_t)(head_dim + 1) * 4;
 }
@@ -596,7 +669,7 @@ extern "C" int acache_shared_prefix_attention(const void* q, int64_t q_stride, v
     return ACACHE_ELIMIT;
   if (max_seqlen_q > total_q) max_seqlen_q = total_q;
   const shared_prefix::Plan plan =
-      shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads);
+      shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads, head_dim);
   const int64_t n_rows = (int64_t)total_q * n_heads, n_parts = plan.prefix_splits + plan.own_splits;
   if (scratch_bytes < n_parts * n_rows * (head_dim + 1) * 4) return ACACHE_EINVAL;
   float* o = (float*)scratch;

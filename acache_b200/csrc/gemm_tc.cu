@@ -13,7 +13,8 @@
 //            tiles would leave most of the 74 pairs idle.  The normalisation kernel that consumes
 //            the projection adds the slices (`acache_add_rmsnorm_partials`).
 //   int8     X and W hold 8-bit integers, the sums are 32-bit integers (exact), and
-//            out[i, j] = acc * x_scale[i] * w_scale[j] (+ bias) in fp32, rounded once
+//            out[i, j] = acc * x_scale[i] * w_scale[j] (+ bias) in fp32, rounded once; with the K
+//            range cut into slices the integer sums go to partial[s] and a second kernel adds them
 //
 // Two CTAs of a cluster work as one: `tcgen05.mma.cta_group::2` multiplies a 256-row block of X
 // (128 rows staged by each CTA) with a BN-column block of W (BN/2 rows staged by each CTA), so a
@@ -31,6 +32,7 @@
 // accumulator stages (when they fit the 512 TMEM columns) the epilogue of a tile overlaps the
 // products of the next.  All waits are bounded; a wait that runs out raises error code 5.
 #include "common.cuh"
+#include "gemm_i8.cuh"
 #include "tcgen05.cuh"
 
 namespace acache {
@@ -450,7 +452,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
           }
         }
         float row_scale = 0.f;
-        if (I8 && live) row_scale = p.x_scale[m];
+        if (I8 && live && p.ksplit == 1) row_scale = p.x_scale[m];
         float run_max = -INFINITY, run_sum = 0.f;
         int run_arg = 0;
 #pragma unroll 1
@@ -470,7 +472,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
             if constexpr (EPI == EPI_PARTIAL) epi_partial(p, ks, m, nn, v);
             if constexpr (EPI == EPI_SWIGLU) epi_swiglu<T>(p, m, nn, v);
             if constexpr (EPI == EPI_QKV) epi_qkv<T, TR, TC>(p, m, nn, v, pos, slot);
-            if constexpr (EPI == EPI_INT8) epi_int8<TR>(p, m, nn, half == 0 ? v0 : v1, row_scale);
+            if constexpr (EPI == EPI_INT8) {
+              if (p.ksplit > 1) epi_partial(p, ks, m, nn, v);      // the bits of the integers
+              else epi_int8<TR>(p, m, nn, half == 0 ? v0 : v1, row_scale);
+            }
             if constexpr (EPI == EPI_ARGMAX) {
               // logits as the unfused projection leaves them (rounded to T); first maximum wins
               float x[16], mx = -INFINITY;
@@ -513,6 +518,38 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   if (warp == 1) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
   }
+}
+
+// ---- the second step of a sliced 8-bit projection: the slices' integer sums added (exactly), scaled and rounded;
+// 8 columns per thread
+template <typename T>
+__global__ void __launch_bounds__(256) int8_fold_kernel(const int32_t* __restrict__ partial, int splits, int M, int N,
+                                                        const float* __restrict__ x_scale, const float* __restrict__ w_scale,
+                                                        const T* __restrict__ bias, T* __restrict__ out, int64_t ldo) {
+  chain_release();
+  chain_wait();
+  const int per_row = N / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(i / per_row), n = (int)(i % per_row) * 8;
+  if (m >= M) return;
+  int32_t acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int s = 0; s < splits; ++s) {
+    const uint4 a = ld_global_nc(partial + ((int64_t)s * M + m) * N + n), b = ld_global_nc(partial + ((int64_t)s * M + m) * N + n + 4);
+    acc[0] += (int32_t)a.x; acc[1] += (int32_t)a.y; acc[2] += (int32_t)a.z; acc[3] += (int32_t)a.w;
+    acc[4] += (int32_t)b.x; acc[5] += (int32_t)b.y; acc[6] += (int32_t)b.z; acc[7] += (int32_t)b.w;
+  }
+  float ws[8], o[8];
+  load8<float>(w_scale + n, ws);
+  const float xs = x_scale[m];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = ((float)acc[e] * xs) * ws[e];
+  if (bias) {
+    float b[8];
+    load8<T>(bias + n, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] += b[e];
+  }
+  *reinterpret_cast<uint4*>(out + (int64_t)m * ldo + n) = pack8<T>(o);
 }
 
 // ---- the second step of the fused output head: fold the per-tile statistics of every row into
@@ -650,6 +687,33 @@ static int plan_splits(int M, int N, int K) {
   if (s > 4) s = 4;
   while (s > 1 && (k_blocks / s < 48 || (s - 1) * ((k_blocks + s - 1) / s) >= k_blocks)) --s;
   return s < 2 ? 1 : (int)s;
+}
+
+// Tile width and K slices of an 8-bit projection (one 256-row block per pair).  Measured on B200: a 128-byte k block
+// takes a pair 0.39 us whatever its tile's width from 64 to 256 columns (97 ns for each of its four products;
+// 512 x 12288 x 4096: 37-38 us at every width from 128 to 256), so wide tiles do more per k block, and with few of them
+// the K range is sliced: the slices' integer sums cost a second kernel (about 3 us) and their traffic (4 TB/s).  Two row
+// blocks per pair were slower everywhere but at 512 x 4096 x 12288 (29.3 against 29.7 us): their epilogue is exposed.
+struct Int8Plan { int bn, splits; };
+static Int8Plan plan_int8(int M, int N, int K, int want_bn) {
+  const int k_blocks = (K + 127) / 128, m_tiles = (M + 255) / 256;
+  double best = 1e30;
+  Int8Plan out{256, 1};
+  for (int bn = 256; bn >= 64; bn -= 32) {
+    if (want_bn && bn != want_bn) continue;
+    const long tiles = (long)m_tiles * ((N + bn - 1) / bn);
+    for (int s = 1; s <= 8; ++s) {
+      const int per = (k_blocks + s - 1) / s;
+      if (s > 1 && (per < 4 || (s - 1) * per >= k_blocks)) continue;       // no empty slice
+      const long waves = (tiles * s + kPairs - 1) / kPairs;
+      const double cost = waves * per * (0.36 + bn * 1e-4) + (s > 1 ? 3.0 + s * 2.0e-6 * M * N : 0.0);
+      if (cost < best * 0.97) {
+        best = cost;
+        out = Int8Plan{bn, s};
+      }
+    }
+  }
+  return out;
 }
 
 }  // namespace gemm
@@ -800,11 +864,20 @@ extern "C" int acache_linear_argmax(const void* x, int64_t x_stride, int n_rows,
   return ACACHE_OK;
 }
 
+extern "C" int64_t acache_linear_int8_scratch_bytes(int n_rows, int in_features, int out_features, int tile_bn) {
+  if (n_rows <= 0 || in_features <= 0 || out_features <= 0 || (tile_bn == 0 && few::takes(n_rows, out_features, in_features)))
+    return 0;
+  const int s = gemm::plan_int8(n_rows, out_features, in_features, tile_bn).splits;
+  return s > 1 ? s * (int64_t)n_rows * out_features * 4 : 0;
+}
+
 extern "C" int acache_linear_int8(const int8_t* x, int64_t x_stride, const float* x_scale, int n_rows, int in_features,
                                   const int8_t* weight, const float* w_scale, int out_features, const void* bias, int dtype,
-                                  void* out, int64_t out_stride, int tile_mb, int tile_bn, int32_t* err_flag, void* stream) {
+                                  void* out, int64_t out_stride, int tile_bn, void* scratch, int64_t scratch_bytes,
+                                  int32_t* err_flag, void* stream) {
   if (n_rows < 0 || in_features <= 0 || out_features <= 0) return ACACHE_EINVAL;
   if (dtype != ACACHE_BF16 && dtype != ACACHE_F16) return ACACHE_EUNSUPPORTED;
+  if (tile_bn != 0 && (tile_bn % 32 != 0 || tile_bn < 64 || tile_bn > 256)) return ACACHE_EINVAL;
   if (n_rows == 0) return ACACHE_OK;
   if (!x || !x_scale || !weight || !w_scale || !out) return ACACHE_EINVAL;
   if (in_features % 16 != 0 || out_features % 16 != 0 || x_stride % 16 != 0 || out_stride % 8 != 0 || !aligned16(x) ||
@@ -812,20 +885,37 @@ extern "C" int acache_linear_int8(const int8_t* x, int64_t x_stride, const float
     return ACACHE_EUNSUPPORTED;
   // |acc| <= 128 * 128 * K has to fit 31 bits
   if (in_features > 131071) return ACACHE_ELIMIT;
-  if ((tile_mb != 0 && tile_mb != 1 && tile_mb != 2) || (tile_bn != 0 && (tile_bn % 32 != 0 || tile_bn < 64 || tile_bn > 256)))
+  if (tile_bn == 0 && few::takes(n_rows, out_features, in_features))
+    return linear_i8_few(few::Params{x, x_stride, x_scale, weight, w_scale, bias, out, out_stride, n_rows, out_features, in_features},
+                         dtype, (cudaStream_t)stream);
+  const gemm::Int8Plan plan = gemm::plan_int8(n_rows, out_features, in_features, tile_bn);
+  if (plan.splits > 1 && (!scratch || !aligned16(scratch) || scratch_bytes < plan.splits * (int64_t)n_rows * out_features * 4))
     return ACACHE_EINVAL;
-  const gemm::Tile tile = gemm::pick_tile(n_rows, out_features, tile_mb, tile_bn, 32, 1.03);
-  if (tile.smem == 0) return ACACHE_EUNSUPPORTED;
+  gemm::Tile tile{1, plan.bn, 0, 2, 0};
+  const int stage_bytes = gemm::A_SUB + plan.bn / 2 * 128;
+  tile.stages = 200 * 1024 / stage_bytes < gemm::kMaxStages ? 200 * 1024 / stage_bytes & ~1 : gemm::kMaxStages;   // handed back in twos
+  tile.smem = (size_t)tile.stages * stage_bytes + 512;
   gemm::Params p{};
-  p.M = n_rows; p.N = out_features; p.K = in_features; p.MB = tile.mb; p.BN = tile.bn; p.stages = tile.stages;
-  p.acc_stages = tile.acc_stages; p.ksplit = 1; p.group = tile.mb == 1 ? 2 : 1;
-  if (p.group == 2 && (p.stages & 1)) p.stages -= 1;
+  p.M = n_rows; p.N = out_features; p.K = in_features; p.MB = 1; p.BN = plan.bn; p.stages = tile.stages;
+  p.acc_stages = 2; p.ksplit = plan.splits; p.group = 2; p.partial = (float*)scratch;
   CUtensorMap mx, mw;
   if (!tc::make_tensor_map_2d_i8(&mx, x, n_rows, in_features, x_stride, 128) ||
-      !tc::make_tensor_map_2d_i8(&mw, weight, out_features, in_features, in_features, tile.bn / 2))
+      !tc::make_tensor_map_2d_i8(&mw, weight, out_features, in_features, in_features, plan.bn / 2))
     return ACACHE_EUNSUPPORTED;
   p.out = out; p.ldo = out_stride; p.bias = bias; p.err_flag = err_flag; p.x_scale = x_scale; p.w_scale = w_scale;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == ACACHE_BF16) return gemm::launch<int8_t, __nv_bfloat16, float, gemm::EPI_INT8>(mx, mw, p, tile, st);
-  return gemm::launch<int8_t, __half, float, gemm::EPI_INT8>(mx, mw, p, tile, st);
+  int rc;
+  if (dtype == ACACHE_BF16) rc = gemm::launch_mb<int8_t, __nv_bfloat16, float, gemm::EPI_INT8, 1>(mx, mw, p, tile, st);
+  else rc = gemm::launch_mb<int8_t, __half, float, gemm::EPI_INT8, 1>(mx, mw, p, tile, st);
+  if (rc != ACACHE_OK || plan.splits == 1) return rc;
+  const int64_t units = (int64_t)n_rows * (out_features / 8);
+  const dim3 grid((unsigned)((units + 255) / 256));
+  if (dtype == ACACHE_BF16)
+    ACACHE_CUDA_CHECK(launch_chained(gemm::int8_fold_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, (const int32_t*)scratch, plan.splits,
+                                     n_rows, out_features, x_scale, w_scale, (const __nv_bfloat16*)bias, (__nv_bfloat16*)out, out_stride));
+  else
+    ACACHE_CUDA_CHECK(launch_chained(gemm::int8_fold_kernel<__half>, grid, dim3(256), 0, st, (const int32_t*)scratch, plan.splits, n_rows,
+                                     out_features, x_scale, w_scale, (const __half*)bias, (__half*)out, out_stride));
+  ACACHE_LAUNCH_CHECK();
+  return ACACHE_OK;
 }

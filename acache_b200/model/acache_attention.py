@@ -195,27 +195,30 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_slots, cu_seqlens_q, cu_
     request are left out of the result (undefined there); a request without any key gets zeros.
 
     ``acache_attention`` reads the prefix once per request, its grouped form once per two requests."""
-    _check_qkv(q, k_cache, v_cache)
-    _require_cuda(prefix_slots, cu_seqlens_q, cu_seqlens_k, read_slot_mapping, prefix_keep)
     total_q, nh, D = q.shape
+    q_stride, *q_inner = q.stride()
+    dev, dtype = q.device, q.dtype
+    assert q.is_cuda and q_inner == [D, 1], "heads of a query row lie side by side"
+    assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape
+    assert k_cache.dtype == dtype and v_cache.dtype == dtype and k_cache.device == dev and v_cache.device == dev
     hkv = k_cache.shape[-2]
-    batch, P = cu_seqlens_q.numel() - 1, prefix_slots.numel()
-    assert k_cache.shape == v_cache.shape and k_cache.shape[-1] == D and nh % hkv == 0
+    batch, P, n_slots = cu_seqlens_q.numel() - 1, prefix_slots.numel(), read_slot_mapping.numel()
+    assert k_cache.shape[-1] == D and nh % hkv == 0
     for t in (prefix_slots, cu_seqlens_q, cu_seqlens_k, read_slot_mapping):
-        assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.device == q.device
+        assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.device == dev
     assert batch >= 0 and cu_seqlens_k.numel() == batch + 1
-    assert k_cache.device == q.device and v_cache.device == q.device
+    keep_stride = 2 * ((P + 63) // 64)
     if prefix_keep is not None:
+        assert prefix_keep.device == dev
         if prefix_keep.dtype == torch.bool:
             assert prefix_keep.shape == (batch, P)
             prefix_keep = pack_keep_mask(prefix_keep)
-        assert prefix_keep.dtype == torch.int32 and prefix_keep.shape == (batch, 2 * ((P + 63) // 64))
-        assert prefix_keep.is_contiguous() and prefix_keep.device == q.device
+        assert prefix_keep.dtype == torch.int32 and prefix_keep.shape == (batch, keep_stride) and prefix_keep.is_contiguous()
         if P == 0:
             prefix_keep = None
     if softmax_scale is None:
         softmax_scale = D ** -0.5
-    out = torch.empty(total_q, nh, D, dtype=q.dtype, device=q.device)
+    out = torch.empty(total_q, nh, D, dtype=dtype, device=dev)
     if total_q == 0 or batch == 0:
         return out
     if max_seqlen_q is None:
@@ -225,17 +228,14 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_slots, cu_seqlens_q, cu_
     lib = _lib.load()
     with on_device_of(q):
         # the call's own scratch: two streams, or two captured graphs, never share it
-        nbytes = lib.acache_shared_prefix_attention_scratch_bytes(total_q, nh, hkv, D, batch, int(max_seqlen_q),
-                                                                  int(max_seqlen_k), P)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        nbytes = lib.acache_shared_prefix_attention_scratch_bytes(total_q, nh, hkv, D, batch, max_seqlen_q, max_seqlen_k, P)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _lib.timed("attention_decode" if ATTENTION_PHASE == "decode" else "attention_refresh", ATTENTION_WORK):
             check(lib.acache_shared_prefix_attention(
-                ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(k_cache), ptr(v_cache), k_cache.numel() // (hkv * D),
-                total_q, nh, hkv, D, dtype_code(q.dtype), ptr(prefix_slots), P, ptr(prefix_keep),
-                prefix_keep.stride(0) if prefix_keep is not None else 0, ptr(cu_seqlens_q), ptr(cu_seqlens_k), batch,
-                int(max_seqlen_q), int(max_seqlen_k), ptr(read_slot_mapping), read_slot_mapping.numel(),
-                float(softmax_scale), ptr(scratch), nbytes, ptr(_lib.err_flag(q.device)), stream_ptr()),
-                "shared_prefix_attention", 3)
+                ptr(q), q_stride, ptr(out), nh * D, ptr(k_cache), ptr(v_cache), k_cache.numel() // (hkv * D), total_q, nh,
+                hkv, D, dtype_code(dtype), ptr(prefix_slots), P, ptr(prefix_keep), keep_stride, ptr(cu_seqlens_q),
+                ptr(cu_seqlens_k), batch, max_seqlen_q, max_seqlen_k, ptr(read_slot_mapping), n_slots, softmax_scale,
+                ptr(scratch), nbytes, ptr(_lib.err_flag(dev)), stream_ptr()), "shared_prefix_attention", 3)
     return out
 
 

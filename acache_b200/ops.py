@@ -342,20 +342,24 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     """``(x int8 [n, in] @ weight int8 [out, in]^T) * x_scale[n, None] * weight_scale[None, out] (+ bias)`` with exact
     32-bit integer sums, rounded once to ``out_dtype`` (bf16 / fp16).  ``in`` and ``out`` are multiples of 16."""
     n, k = _rows_of(x)
-    N = weight.shape[0]
+    N, dev = weight.shape[0], x.device
     assert x.dtype == torch.int8 and weight.dtype == torch.int8 and weight.shape == (N, k) and weight.is_contiguous()
     assert x_scale.shape == (n,) and x_scale.dtype == torch.float32 and x_scale.is_contiguous()
     assert weight_scale.shape == (N,) and weight_scale.dtype == torch.float32 and weight_scale.is_contiguous()
-    assert weight.device == x.device and x_scale.device == x.device and weight_scale.device == x.device
+    assert weight.device == dev and x_scale.device == dev and weight_scale.device == dev
     if bias is not None:
-        assert bias.shape == (N,) and bias.dtype == out_dtype and bias.is_contiguous() and bias.device == x.device
-    out = torch.empty(n, N, dtype=out_dtype, device=x.device)
+        assert bias.shape == (N,) and bias.dtype == out_dtype and bias.is_contiguous() and bias.device == dev
+    out = torch.empty(n, N, dtype=out_dtype, device=dev)
     if n:
+        lib = _lib.load()
         with on_device_of(x):
-            check(_lib.load().acache_linear_int8(
+            # the sums of K slices, where the launch cuts the K range: a tensor of this call's own
+            nbytes = lib.acache_linear_int8_scratch_bytes(n, k, N, GEMM_TILE[1])
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            check(lib.acache_linear_int8(
                 ptr(x), x.stride(0), ptr(x_scale), n, k, ptr(weight), ptr(weight_scale), N, ptr(bias), dtype_code(out_dtype),
-                ptr(out), out.stride(0), GEMM_TILE[0], GEMM_TILE[1], ptr(_lib.err_flag(x.device)), stream_ptr()),
-                "linear_int8")
+                ptr(out), N, GEMM_TILE[1], ptr(scratch), nbytes, ptr(_lib.err_flag(dev)), stream_ptr()), "linear_int8",
+                2 if nbytes else 1)
     return out
 
 
@@ -415,33 +419,35 @@ def rope_append(q, k, v, positions, inv_freq, k_cache=None, v_cache=None, slot_m
     ``(q, k)``.  ``interleaved``: pairs (2j, 2j + 1) instead of (j, j + rotary_dim / 2).  ``attention_factor``
     multiplies sine and cosine.  The table form of the half layout over the whole head is ``rope_store``."""
     n, nh, D = q.shape
-    hkv = k.shape[1]
-    assert q.is_cuda and k.shape == (n, hkv, D) and k.dtype == q.dtype and k.device == q.device
-    assert q.stride(2) == 1 and q.stride(1) == D and k.stride(2) == 1 and k.stride(1) == D
-    assert positions.dtype == torch.int64 and positions.shape == (n,) and positions.is_contiguous() and positions.device == q.device
-    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == q.device
-    assert 2 * inv_freq.numel() <= D, "more frequencies than pairs in a head"
-    out_q = torch.empty(n, nh, D, dtype=q.dtype, device=q.device)
-    num_slots, out_k = 0, None
+    hkv, dtype, dev = k.shape[1], q.dtype, q.device
+    (q_stride, *q_inner), (k_stride, *k_inner) = q.stride(), k.stride()
+    assert q.is_cuda and k.shape == (n, hkv, D) and k.dtype == dtype and k.device == dev
+    assert q_inner == [D, 1] and k_inner == [D, 1], "heads of a row lie side by side"
+    assert positions.dtype == torch.int64 and positions.shape == (n,) and positions.is_contiguous() and positions.device == dev
+    half = inv_freq.numel()
+    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev
+    assert 2 * half <= D, "more frequencies than pairs in a head"
+    out_q = torch.empty(n, nh, D, dtype=dtype, device=dev)
+    num_slots, out_k, v_stride = 0, None, 0
     if slot_mapping is not None:
-        assert v is not None and v.shape == k.shape and v.dtype == q.dtype and v.device == q.device
-        assert v.stride(2) == 1 and v.stride(1) == D
+        v_stride, *v_inner = v.stride()
+        assert v.shape == k.shape and v.dtype == dtype and v.device == dev and v_inner == [D, 1]
         assert slot_mapping.dtype == torch.int32 and slot_mapping.shape == (n,) and slot_mapping.is_contiguous()
-        assert slot_mapping.device == q.device and k_cache.device == q.device and v_cache.device == q.device
+        assert slot_mapping.device == dev and k_cache.device == dev and v_cache.device == dev
         assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape
-        assert k_cache.dtype == q.dtype and v_cache.dtype == q.dtype and k_cache.shape[-2:] == (hkv, D)
+        assert k_cache.dtype == dtype and v_cache.dtype == dtype and k_cache.shape[-2:] == (hkv, D)
         num_slots = k_cache.numel() // (hkv * D)
     else:
         assert k_cache is None and v_cache is None, "caches without slot_mapping"
-        out_k = torch.empty(n, hkv, D, dtype=q.dtype, device=q.device)
+        out_k = torch.empty(n, hkv, D, dtype=dtype, device=dev)
         v = None
     if n:
         with on_device_of(q):
             check(_lib.load().acache_rope_append(
-                ptr(q), q.stride(0), ptr(k), k.stride(0), ptr(v), v.stride(0) if v is not None else 0, n, nh, hkv, D,
-                dtype_code(q.dtype), ptr(positions), ptr(inv_freq), 2 * inv_freq.numel(), int(bool(interleaved)),
-                float(attention_factor), ptr(out_q), out_q.stride(0), ptr(k_cache if out_k is None else out_k),
-                ptr(v_cache), ptr(slot_mapping), num_slots, ptr(_lib.err_flag(q.device)), stream_ptr()), "rope_append")
+                ptr(q), q_stride, ptr(k), k_stride, ptr(v), v_stride, n, nh, hkv, D, dtype_code(dtype), ptr(positions),
+                ptr(inv_freq), 2 * half, 1 if interleaved else 0, attention_factor, ptr(out_q), nh * D,
+                ptr(k_cache if out_k is None else out_k), ptr(v_cache), ptr(slot_mapping), num_slots,
+                ptr(_lib.err_flag(dev)), stream_ptr()), "rope_append")
     return out_q if out_k is None else (out_q, out_k)
 
 

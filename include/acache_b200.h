@@ -180,8 +180,10 @@ ACACHE_API int acache_linear_argmax(const void* x, int64_t x_stride, int n_rows,
  * sums exact in 32-bit integers, the rest in fp32, rounded once to dtype (fp16 / bf16, the type of out
  * and bias).  x rows are x_stride bytes apart, weight[out_features, in_features] is dense; in_features and
  * out_features multiples of 16, 16-byte aligned pointers, x_stride a multiple of 16, out_stride of 8, else
- * ACACHE_EUNSUPPORTED; in_features above 131071 could overflow the sums: ACACHE_ELIMIT.  tile_mb / tile_bn
- * (0 = chosen per launch; tile_bn a multiple of 32 in 64..256) as for acache_linear.
+ * ACACHE_EUNSUPPORTED; in_features above 131071 could overflow the sums: ACACHE_ELIMIT.  tile_bn: columns of a
+ * tile, a multiple of 32 in 64..256, or 0 = chosen per launch.  scratch holds
+ * acache_linear_int8_scratch_bytes() of the same sizes (0 = none needed; sums of K slices, contents irrelevant)
+ * and belongs to the call until it has run.
  *
  * The three quantising producers write q[n_rows, n_cols] dense and one scale per row: scale = a / 127 and
  * q = round(127 y / a), ties to even, with a the largest |y| of the row.  A row of zeros gets scale 0, a row
@@ -198,7 +200,9 @@ ACACHE_API int acache_act_mul_halves_int8(const void* x, int64_t x_stride, int n
                                           int8_t* q, float* scale, void* stream);
 ACACHE_API int acache_linear_int8(const int8_t* x, int64_t x_stride, const float* x_scale, int n_rows, int in_features,
                                   const int8_t* weight, const float* w_scale, int out_features, const void* bias, int dtype,
-                                  void* out, int64_t out_stride, int tile_mb, int tile_bn, int32_t* err_flag, void* stream);
+                                  void* out, int64_t out_stride, int tile_bn, void* scratch, int64_t scratch_bytes,
+                                  int32_t* err_flag, void* stream);
+ACACHE_API int64_t acache_linear_int8_scratch_bytes(int n_rows, int in_features, int out_features, int tile_bn);
 
 /* ------------------------------------------------------------------ rotary positions from frequencies
  * acache_rope_store's job without tables (no counterpart in the reference): q[n, n_heads, head_dim] and

@@ -14,12 +14,12 @@ def test_entry_points_validate_without_a_gpu():
     assert lib.acache_quantize_rows(None, 0, 1, 64, 2, None, None, None) == -1            # null pointers
     assert lib.acache_rmsnorm_int8(None, 0, None, 0, None, 1, 0, 1e-5, 2, None, None, None) == -1
     assert lib.acache_act_mul_halves_int8(None, 0, 1, 64, 3, 2, None, None, None) == -1   # activation
-    assert lib.acache_linear_int8(None, 0, None, 0, 64, None, None, 64, None, 2, None, 0, 0, 0, None, None) == 0
-    assert lib.acache_linear_int8(None, 0, None, 1, 64, None, None, 64, None, 0, None, 0, 0, 0, None, None) == -2  # fp32 out
-    assert lib.acache_linear_int8(None, 0, None, 1, 64, None, None, 64, None, 2, None, 0, 0, 0, None, None) == -1
+    assert lib.acache_linear_int8(None, 0, None, 0, 64, None, None, 64, None, 2, None, 0, 0, None, 0, None, None) == 0
+    assert lib.acache_linear_int8(None, 0, None, 1, 64, None, None, 64, None, 0, None, 0, 0, None, 0, None, None) == -2  # fp32 out
+    assert lib.acache_linear_int8(None, 0, None, 1, 64, None, None, 64, None, 2, None, 0, 0, None, 0, None, None) == -1
     bad = 1 << 20                                                                         # never dereferenced
-    assert lib.acache_linear_int8(bad, 64, bad, 1, 72, bad, bad, 64, None, 2, bad, 64, 0, 0, None, None) == -2
-    assert lib.acache_linear_int8(bad, 64, bad, 1, 131072, bad, bad, 64, None, 2, bad, 64, 0, 0, None, None) == -4
+    assert lib.acache_linear_int8(bad, 64, bad, 1, 72, bad, bad, 64, None, 2, bad, 64, 0, None, 0, None, None) == -2
+    assert lib.acache_linear_int8(bad, 64, bad, 1, 131072, bad, bad, 64, None, 2, bad, 64, 0, None, 0, None, None) == -4
     rope = [None, 0, None, 0, None, 0, 1, 2, 1, 64, 2, None, None, 64, 0, 1.0, None, 0, None, None, None, 0, None, None]
     assert lib.acache_rope_append(*rope) == -1
     rope[6] = 0
