@@ -16,9 +16,11 @@
 // A row that holds an infinity or a NaN gets the scale NaN and zeros, so that everything computed
 // from it is NaN; a row of zeros gets the scale 0.
 //
-// One CTA per row, one pass over global memory (the row stays in registers); bound by HBM, in
-// practice by latency at the few hundred rows of a decode step.
+// A CTA works on a row at a time, one pass over global memory (the row stays in registers), and while it reduces
+// and rounds one row the next one it will take is on its way.  Bound by HBM at size, by latency at the few hundred rows
+// of a decode step: gate 2304 x 12288 28 us (5.0 TB/s), 512 x 12288 8.9 us; norm 4096 x 3584 16 us, 512 x 4096 3.9 us.
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace acache {
 namespace quant {
@@ -27,12 +29,12 @@ enum { SRC_ROWS = 0, SRC_NORM = 1, SRC_GATE = 2 };
 
 struct Params {
   const void* x; int64_t x_stride; const void* delta; int64_t d_stride; const void* weight; float eps; int act;
-  int8_t* q; float* scale; int n_cols;
+  int8_t* q; float* scale; int n_rows, n_cols;
 };
 
 __device__ __forceinline__ float act_fn(float x, int act) {
   // the fast exponential and division (a few units of 2^-22): the value is rounded to 8 bits next, and the exact
-  // forms made the kernel bound by instructions (512 x 12288: 14 us against @T_GATE@)
+  // forms made the kernel bound by instructions (512 x 12288: 14 us against 9)
   if (act == 0) return __fdividef(x, 1.f + __expf(-x));
   if (act == 1) return x > 0.f ? x : (x == x ? 0.f : x);      // a NaN stays
   return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
@@ -54,11 +56,11 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits, float* scale_ou
   return r;
 }
 
-__device__ __forceinline__ int quantise(float v, const RowScale& r) {
+// the quantised value in the low byte (of a row that is not dead)
+__device__ __forceinline__ uint32_t quantise(float v, const RowScale& r) {
   float t = (v * r.pre) * r.f;
   t = __uint_as_float((__float_as_uint(t) + 4u) & ~7u);     // 21 significant bits
-  const int q = (int)(__float_as_uint(t + 0x1.8p23f) & 0xFFu);
-  return r.dead ? 0 : q;
+  return __float_as_uint(t + 0x1.8p23f);
 }
 
 template <int NT>
@@ -84,82 +86,108 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return s;
 }
 
+// CTAs per SM the kernel is compiled and launched for
+constexpr int resident(int nt, int vpt) { return vpt == 1 ? 1536 / nt : (vpt == 2 ? 1280 / nt : (vpt <= 4 ? 1024 / nt : 1)); }
+
 template <typename T, int SRC, int NT, int VPT>
-__global__ void __launch_bounds__(NT, VPT <= 4 ? 1024 / NT : 1) quantise_kernel(const Params p) {
+__global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const Params p) {
   constexpr int E = 16 / sizeof(T);
+  constexpr bool TWO = SRC != SRC_ROWS;           // a second input row: up halves, or the residual update
   chain_release();
   chain_wait();
+  // a thread's vectors of the next row, on their way while it works on the current one (they are its own: no barrier)
+  extern __shared__ __align__(16) uint4 next_row[];      // [TWO ? 2 : 1][VPT][NT]
   __shared__ float red_sum[NT / 32];
-  __shared__ uint32_t red_max[NT / 32];
-  const int64_t row = blockIdx.x;
-  T* xr = (T*)p.x + row * p.x_stride;
-  const int nvec = p.n_cols / E;
-  float y[VPT][E];
-  Vec16<T> w[VPT];                                // the norm's weights, loaded along with the row
-  uint32_t top = 0;
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = threadIdx.x + i * NT;
-    if (c < nvec) {
-      Vec16<T> a;
-      a.u = *reinterpret_cast<const uint4*>(xr + (int64_t)c * E);
-      if (SRC == SRC_NORM) w[i].u = *reinterpret_cast<const uint4*>((const T*)p.weight + (int64_t)c * E);
-      if (SRC == SRC_NORM && p.delta) {           // the residual add, rounded to T, written back
-        Vec16<T> b;
-        b.u = ld_global_nc((const T*)p.delta + row * p.d_stride + (int64_t)c * E);
-#pragma unroll
-        for (int e = 0; e < E; ++e) a.e[e] = from_f32<T>(to_f32<T>(a.e[e]) + to_f32<T>(b.e[e]));
-        *reinterpret_cast<uint4*>(xr + (int64_t)c * E) = a.u;
-      }
-      if (SRC == SRC_GATE) {
-        Vec16<T> b;
-        b.u = *reinterpret_cast<const uint4*>(xr + p.n_cols + (int64_t)c * E);
-#pragma unroll
-        for (int e = 0; e < E; ++e) y[i][e] = act_fn(to_f32<T>(a.e[e]), p.act) * to_f32<T>(b.e[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          y[i][e] = to_f32<T>(a.e[e]);
-          if (SRC == SRC_NORM) ss = fmaf(y[i][e], y[i][e], ss);
-        }
-      }
-      if (SRC != SRC_NORM) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) top = max(top, abs_bits(y[i][e]));
-      }
-    }
-  }
-  if (SRC == SRC_NORM) {
-    const float rs = rsqrtf(block_sum<NT>(ss, red_sum) / (float)p.n_cols + p.eps);
+  __shared__ uint32_t red_max[2][NT / 32];
+  const int tid = threadIdx.x, nvec = p.n_cols / E;
+  const bool two = SRC == SRC_GATE || (SRC == SRC_NORM && p.delta);
+  auto fetch = [&](int64_t row) {
+    const T* xr = (const T*)p.x + row * p.x_stride;
+    const T* yr = SRC == SRC_GATE ? xr + p.n_cols : (const T*)p.delta + row * p.d_stride;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = threadIdx.x + i * NT;
+      const int c = tid + i * NT;
       if (c < nvec) {
+        tc::cp_async16(tc::smem_u32(next_row + i * NT + tid), xr + (int64_t)c * E, true);
+        if (TWO && two) tc::cp_async16(tc::smem_u32(next_row + (VPT + i) * NT + tid), yr + (int64_t)c * E, true);
+      }
+    }
+    tc::cp_async_commit();
+  };
+  int64_t row = blockIdx.x;
+  fetch(row);
+  Vec16<T> w[VPT];                                // the norm's weights
+  if (SRC == SRC_NORM) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          y[i][e] = y[i][e] * rs * to_f32<T>(w[i].e[e]);
-          top = max(top, abs_bits(y[i][e]));
+    for (int i = 0; i < VPT; ++i)
+      if (tid + i * NT < nvec) w[i].u = *reinterpret_cast<const uint4*>((const T*)p.weight + (int64_t)(tid + i * NT) * E);
+  }
+  for (int parity = 0; row < p.n_rows; row += gridDim.x, parity ^= 1) {
+    T* xr = (T*)p.x + row * p.x_stride;
+    float y[VPT][E];
+    uint32_t top = 0;
+    float ss = 0.f;
+    tc::cp_async_wait<0>();
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = tid + i * NT;
+      if (c < nvec) {
+        Vec16<T> a, b;
+        a.u = next_row[i * NT + tid];
+        if (TWO && two) b.u = next_row[(VPT + i) * NT + tid];
+        if (SRC == SRC_NORM && two) {             // the residual add, rounded to T, written back
+#pragma unroll
+          for (int e = 0; e < E; ++e) a.e[e] = from_f32<T>(to_f32<T>(a.e[e]) + to_f32<T>(b.e[e]));
+          *reinterpret_cast<uint4*>(xr + (int64_t)c * E) = a.u;
+        }
+        if (SRC == SRC_GATE) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) y[i][e] = act_fn(to_f32<T>(a.e[e]), p.act) * to_f32<T>(b.e[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            y[i][e] = to_f32<T>(a.e[e]);
+            if (SRC == SRC_NORM) ss = fmaf(y[i][e], y[i][e], ss);
+          }
+        }
+        if (SRC != SRC_NORM) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) top = max(top, abs_bits(y[i][e]));
         }
       }
     }
-  }
-  top = block_max<NT>(top, red_max);
-  const RowScale r = row_scale(top, threadIdx.x == 0 ? p.scale + row : nullptr);
-  int8_t* qr = p.q + row * p.n_cols;
+    if (row + gridDim.x < p.n_rows) fetch(row + gridDim.x);
+    if (SRC == SRC_NORM) {
+      const float rs = rsqrtf(block_sum<NT>(ss, red_sum) / (float)p.n_cols + p.eps);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = threadIdx.x + i * NT;
-    if (c < nvec) {
-      uint32_t word[E / 4];
+      for (int i = 0; i < VPT; ++i) {
+        if (tid + i * NT < nvec) {
 #pragma unroll
-      for (int g = 0; g < E / 4; ++g) {
-        word[g] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) word[g] |= (uint32_t)quantise(y[i][4 * g + e], r) << (8 * e);
+          for (int e = 0; e < E; ++e) {
+            y[i][e] = y[i][e] * rs * to_f32<T>(w[i].e[e]);
+            top = max(top, abs_bits(y[i][e]));
+          }
+        }
       }
-      if (E == 8) *reinterpret_cast<uint2*>(qr + (int64_t)c * E) = make_uint2(word[0], word[E / 4 - 1]);
-      else *reinterpret_cast<uint32_t*>(qr + (int64_t)c * E) = word[0];
+    }
+    top = block_max<NT>(top, red_max[parity]);    // two buffers: a fast warp may be one row ahead of a slow one
+    const RowScale r = row_scale(top, tid == 0 ? p.scale + row : nullptr);
+    int8_t* qr = p.q + row * p.n_cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = tid + i * NT;
+      if (c < nvec) {
+        uint32_t word[E / 4];
+#pragma unroll
+        for (int g = 0; g < E / 4; ++g) {
+          const float* v = &y[i][4 * g];
+          word[g] = __byte_perm(__byte_perm(quantise(v[0], r), quantise(v[1], r), 0x0040),
+                                __byte_perm(quantise(v[2], r), quantise(v[3], r), 0x0040), 0x5410);
+          if (r.dead) word[g] = 0;
+        }
+        if (E == 8) *reinterpret_cast<uint2*>(qr + (int64_t)c * E) = make_uint2(word[0], word[E / 4 - 1]);
+        else *reinterpret_cast<uint32_t*>(qr + (int64_t)c * E) = word[0];
+      }
     }
   }
 }
@@ -197,26 +225,38 @@ __global__ void __launch_bounds__(256) quantise_any_kernel(const Params p) {
   top = block_max<256>(top, red_max);
   const RowScale r = row_scale(top, threadIdx.x == 0 ? p.scale + row : nullptr);
   int8_t* qr = p.q + row * p.n_cols;
-  for (int c = threadIdx.x; c < p.n_cols; c += 256) qr[c] = (int8_t)quantise(value(c), r);
+  for (int c = threadIdx.x; c < p.n_cols; c += 256) qr[c] = r.dead ? (int8_t)0 : (int8_t)(quantise(value(c), r) & 0xFFu);
+}
+
+template <typename T, int SRC, int NT, int VPT>
+static int launch_row(const Params& p, cudaStream_t st) {
+  constexpr size_t smem = (size_t)(SRC == SRC_ROWS ? 1 : 2) * VPT * NT * 16;
+  auto kern = quantise_kernel<T, SRC, NT, VPT>;
+  if (smem > 48 * 1024) ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const int64_t most = (int64_t)kNumSMs * resident(NT, VPT);
+  ACACHE_CUDA_CHECK(launch_chained(kern, dim3((unsigned)(p.n_rows < most ? p.n_rows : most)), dim3(NT), smem, st, p));
+  ACACHE_LAUNCH_CHECK();
+  return ACACHE_OK;
 }
 
 template <typename T, int SRC>
-static int launch(const Params& p, int64_t n_rows, cudaStream_t st) {
+static int launch(const Params& p, cudaStream_t st) {
   constexpr int E = 16 / sizeof(T);
   const bool vec = p.n_cols % E == 0 && p.x_stride % E == 0 && aligned16(p.x) && (!p.delta || (p.d_stride % E == 0 && aligned16(p.delta))) &&
                    (!p.weight || aligned16(p.weight)) && (reinterpret_cast<uintptr_t>(p.q) & 7) == 0;
   const int nvec = p.n_cols / E;
-  const dim3 grid((unsigned)n_rows);
   // the row in registers: at most 8 vectors of 8 values a thread; wider rows are read again instead
-  if (!vec || nvec > 4096) ACACHE_CUDA_CHECK(launch_chained(quantise_any_kernel<T, SRC>, grid, dim3(256), 0, st, p));
-  else if (nvec <= 128) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 128, 1>, grid, dim3(128), 0, st, p));
-  else if (nvec <= 256) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 256, 1>, grid, dim3(256), 0, st, p));
-  else if (nvec <= 512) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 256, 2>, grid, dim3(256), 0, st, p));
-  else if (nvec <= 1024) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 512, 2>, grid, dim3(512), 0, st, p));
-  else if (nvec <= 2048) ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 512, 4>, grid, dim3(512), 0, st, p));
-  else ACACHE_CUDA_CHECK(launch_chained(quantise_kernel<T, SRC, 512, 8>, grid, dim3(512), 0, st, p));
-  ACACHE_LAUNCH_CHECK();
-  return ACACHE_OK;
+  if (!vec || nvec > 4096) {
+    ACACHE_CUDA_CHECK(launch_chained(quantise_any_kernel<T, SRC>, dim3(p.n_rows), dim3(256), 0, st, p));
+    ACACHE_LAUNCH_CHECK();
+    return ACACHE_OK;
+  }
+  if (nvec <= 128) return launch_row<T, SRC, 128, 1>(p, st);
+  if (nvec <= 256) return launch_row<T, SRC, 256, 1>(p, st);
+  if (nvec <= 512) return launch_row<T, SRC, 256, 2>(p, st);
+  if (nvec <= 1024) return launch_row<T, SRC, 256, 4>(p, st);
+  if (nvec <= 2048) return launch_row<T, SRC, 512, 4>(p, st);
+  return launch_row<T, SRC, 512, 8>(p, st);
 }
 
 }  // namespace quant
@@ -229,8 +269,8 @@ extern "C" int acache_quantize_rows(const void* x, int64_t x_stride, int n_rows,
   if (!dtype_ok(dtype) || n_rows < 0 || n_cols <= 0) return ACACHE_EINVAL;
   if (n_rows == 0) return ACACHE_OK;
   if (!x || !q || !scale) return ACACHE_EINVAL;
-  const quant::Params p{x, x_stride, nullptr, 0, nullptr, 0.f, 0, q, scale, n_cols};
-  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_ROWS>(p, n_rows, (cudaStream_t)stream)));
+  const quant::Params p{x, x_stride, nullptr, 0, nullptr, 0.f, 0, q, scale, n_rows, n_cols};
+  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_ROWS>(p, (cudaStream_t)stream)));
   return ACACHE_EINVAL;
 }
 
@@ -239,8 +279,8 @@ extern "C" int acache_rmsnorm_int8(void* x, int64_t x_stride, const void* delta,
   if (!dtype_ok(dtype) || n_rows < 0 || n_cols <= 0) return ACACHE_EINVAL;
   if (n_rows == 0) return ACACHE_OK;
   if (!x || !weight || !q || !scale) return ACACHE_EINVAL;
-  const quant::Params p{x, x_stride, delta, d_stride, weight, eps, 0, q, scale, n_cols};
-  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_NORM>(p, n_rows, (cudaStream_t)stream)));
+  const quant::Params p{x, x_stride, delta, d_stride, weight, eps, 0, q, scale, n_rows, n_cols};
+  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_NORM>(p, (cudaStream_t)stream)));
   return ACACHE_EINVAL;
 }
 
@@ -249,7 +289,7 @@ extern "C" int acache_act_mul_halves_int8(const void* x, int64_t x_stride, int n
   if (!dtype_ok(dtype) || n_rows < 0 || ffn <= 0 || act < 0 || act > 2) return ACACHE_EINVAL;
   if (n_rows == 0) return ACACHE_OK;
   if (!x || !q || !scale) return ACACHE_EINVAL;
-  const quant::Params p{x, x_stride, nullptr, 0, nullptr, 0.f, act, q, scale, ffn};
-  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_GATE>(p, n_rows, (cudaStream_t)stream)));
+  const quant::Params p{x, x_stride, nullptr, 0, nullptr, 0.f, act, q, scale, n_rows, ffn};
+  ACACHE_DISPATCH_DTYPE(dtype, T, return (quant::launch<T, quant::SRC_GATE>(p, (cudaStream_t)stream)));
   return ACACHE_EINVAL;
 }
