@@ -1,6 +1,6 @@
 // Shared-prefix attention is computed in parts (a range of keys for a set of rows) that are merged at the
 // end: the description of a segment (the shared prefix, or the requests' own keys) that the kernels of
-// attention_shared.cu and the split form of attention_tc256.cu have in common.
+// attention_shared.cu and attention_shared_wide.cu have in common.
 #pragma once
 #include "common.cuh"
 
@@ -58,6 +58,6 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int n_req, int q) {
 
 }  // namespace parts
 
-int attention_tc256_parts(const parts::Args& a, const parts::Seg& seg, int n_requests, int max_q);
+int attention_wide_parts(const parts::Args& a, const parts::Seg& seg, int n_requests, int max_q);
 
 }  // namespace acache

@@ -8,7 +8,7 @@
 // rows of ALL requests, own parts over each request's rows), each part yields (O / l, log2 of its sum), and a
 // row's parts are merged at the end:  o = sum_p 2^(lse_p - top) O_p / sum_p 2^(lse_p - top).
 //
-// A part whose rows fill the tensor cores' 128-row tiles goes to the split form of attention_tc256.cu
+// A part whose rows fill the tensor cores' 128-row tiles goes to attention_shared_wide.cu
 // (tcgen05, 256 rows share a staged K/V tile).  A part with few rows (single tokens, short blocks: bound by
 // the bytes of K and V) goes to rows_kernel below.
 //
@@ -26,8 +26,6 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 
-#include <math.h>
-
 namespace acache {
 namespace shared_prefix {
 
@@ -38,7 +36,6 @@ using tc::ex2;
 using tc::pack2;
 using tc::smem_u32;
 
-constexpr int NG = 4;                 // key groups of a CTA
 constexpr int KB = 16;                // keys of a block
 constexpr int NS = 3;                 // stages of a group's ring
 
@@ -246,18 +243,18 @@ __device__ __forceinline__ void finish_rows(const parts::Args& a, const parts::S
   }
 }
 
-// FINAL: the segment is the requests' own keys in one range each: the CTA also merges the prefix parts (written by
-// the kernel before it in the stream, beside which it may run) and writes the output.  Else it leaves a part.
-template <typename T, int D, int RT, bool FINAL>
-__global__ void __launch_bounds__(RT * NG * 32, 2) rows_kernel(const __grid_constant__ parts::Args a, const __grid_constant__ parts::Seg s,
+// final: the segment is the requests' own keys in one range each and the CTA also merges the prefix parts (written by
+// the kernel before it in the stream, beside which it may run) and writes the output; else it leaves a part.
+// NG: key groups of a CTA, 4 or 2; both keep 16 warps (two row tiles) on an SM, two groups make more and longer CTAs.
+template <typename T, int D, int RT, int NG>
+__global__ void __launch_bounds__(RT * NG * 32, 8 / NG) rows_kernel(const __grid_constant__ parts::Args a, const __grid_constant__ parts::Seg s,
                                                                const __grid_constant__ parts::Seg prefix,
-                                                               const __grid_constant__ Merge mg, int beside) {
+                                                               const __grid_constant__ Merge mg, int beside, int final) {
   constexpr int NT = RT * NG * 32, ROWS = RT * 16, CH = D / 8, KS = D / 16, E = D / 32;
   constexpr int BLOCK = KB * D * 2;             // bytes of K (or V) of a block
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* sQ = smem;                           // [ROWS][D]
   uint8_t* ring = smem + ROWS * D * 2;          // [NG][NS][K | V]
-  __shared__ float s_m[NG][ROWS], s_l[NG][ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int grp = warp % NG, rt = warp / NG;    // key group and row tile of the warp
 
@@ -440,7 +437,10 @@ __global__ void __launch_bounds__(RT * NG * 32, 2) rows_kernel(const __grid_cons
   // ---- the groups' results through shared memory (over the ring)
   __syncthreads();
   constexpr int LD = D + 8;                     // rows 8 banks apart: the float2 stores of a half warp do not collide
-  float* sO = reinterpret_cast<float*>(ring);   // [NG][ROWS][LD]
+  float* sO = reinterpret_cast<float*>(ring);   // [NG][ROWS][LD], then the groups' maxima and sums [NG][ROWS]
+  static_assert(NG * ROWS * (LD + 2) * 4 <= NG * NS * 2 * BLOCK, "the exchange lies over the ring");
+  float* s_m = sO + NG * ROWS * LD;
+  float* s_l = s_m + NG * ROWS;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int row = rt * 16 + lane / 4 + 8 * h;
@@ -448,84 +448,98 @@ __global__ void __launch_bounds__(RT * NG * 32, 2) rows_kernel(const __grid_cons
     l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
     l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
     if ((lane & 3) == 0) {
-      s_m[grp][row] = m_ref[h];
-      s_l[grp][row] = l;
+      s_m[grp * ROWS + row] = m_ref[h];
+      s_l[grp * ROWS + row] = l;
     }
 #pragma unroll
     for (int d = 0; d < D / 8; ++d)
       *reinterpret_cast<float2*>(sO + (grp * ROWS + row) * LD + d * 8 + 2 * (lane & 3)) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
   }
   __syncthreads();
-  if (beside) chain_wait();                     // the prefix parts are there
-  constexpr int N = 4;                          // rows of a warp: warp, warp + NW, ...
-  float acc[N][E], m[N], l[N];
-  int q_row[N], head[N];
-  bool live[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int row = warp + n * (RT * NG), vr = m0 + row;
-    live[n] = vr < vrows;
-    q_row[n] = r.q0 + (live[n] ? vr / g : 0);
-    head[n] = kvh * g + (live[n] ? vr % g : 0);
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int w = 0; w < NG; ++w) m[n] = fmaxf(m[n], s_m[w][row]);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < NG; ++w) {
-      const float mw = s_m[w][row], lw = s_l[w][row];
-      const bool none = mw == -INFINITY && lw == 0.f;        // no key (only NaN scores leave a NaN sum)
-      const float f = none ? 0.f : ex2(mw - m[n]);
-      l[n] = fmaf(f, lw, l[n]);
-      float x[E];
-      const float* src = sO + (w * ROWS + row) * LD + lane * E;
-      if constexpr (E == 4) {
-        const float4 t = *reinterpret_cast<const float4*>(src);
-        x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
-      } else {
-        const float2 t = *reinterpret_cast<const float2*>(src);
-        x[0] = t.x; x[1] = t.y;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[n][e] = none ? acc[n][e] : fmaf(f, x[e], acc[n][e]);
-    }
-  }
-  if constexpr (FINAL) {
-    finish_rows<T, D, N>(a, s, prefix, mg, s.first_part, s.first_part, q_row, head, live, acc, m, l);
-  } else {
+  if (beside && final) chain_wait();            // the prefix parts are there
+  constexpr int N = 4;                          // rows that a warp finishes together
+#pragma unroll 1
+  for (int row0 = warp; row0 < ROWS; row0 += N * RT * NG) {
+    float acc[N][E], m[N], l[N];
+    int q_row[N], head[N];
+    bool live[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      if (!live[n]) continue;
-      const int64_t at_row = (int64_t)(s.first_part + split) * s.n_rows + (int64_t)q_row[n] * a.n_heads + head[n];
-      const bool any_key = m[n] != -INFINITY || l[n] != 0.f;
-      if (any_key) {
-        const float inv = 1.f / l[n];
-        float* dst = s.o + at_row * D + lane * E;
-        if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc[n][0] * inv, acc[n][1] * inv, acc[n][2] * inv, acc[n][3] * inv);
-        else *reinterpret_cast<float2*>(dst) = make_float2(acc[n][0] * inv, acc[n][1] * inv);
+      const int row = row0 + n * (RT * NG), vr = m0 + row;
+      live[n] = row < ROWS && vr < vrows;
+      q_row[n] = r.q0 + (live[n] ? vr / g : 0);
+      head[n] = kvh * g + (live[n] ? vr % g : 0);
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NG; ++w) m[n] = fmaxf(m[n], s_m[w * ROWS + (row & (ROWS - 1))]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NG; ++w) {
+        const float mw = s_m[w * ROWS + (row & (ROWS - 1))], lw = s_l[w * ROWS + (row & (ROWS - 1))];
+        const bool none = mw == -INFINITY && lw == 0.f;        // no key (only NaN scores leave a NaN sum)
+        const float f = none ? 0.f : ex2(mw - m[n]);
+        l[n] = fmaf(f, lw, l[n]);
+        float x[E];
+        const float* src = sO + (w * ROWS + (row & (ROWS - 1))) * LD + lane * E;
+        if constexpr (E == 4) {
+          const float4 t = *reinterpret_cast<const float4*>(src);
+          x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+        } else {
+          const float2 t = *reinterpret_cast<const float2*>(src);
+          x[0] = t.x; x[1] = t.y;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[n][e] = none ? acc[n][e] : fmaf(f, x[e], acc[n][e]);
       }
-      if (lane == 0) s.lse[at_row] = any_key ? m[n] + log2f(l[n]) : -INFINITY;
+    }
+    if (final) {
+      finish_rows<T, D, N>(a, s, prefix, mg, s.first_part, s.first_part, q_row, head, live, acc, m, l);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (!live[n]) continue;
+        const int64_t at_row = (int64_t)(s.first_part + split) * s.n_rows + (int64_t)q_row[n] * a.n_heads + head[n];
+        const bool any_key = m[n] != -INFINITY || l[n] != 0.f;
+        if (any_key) {
+          const float inv = 1.f / l[n];
+          float* dst = s.o + at_row * D + lane * E;
+          if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc[n][0] * inv, acc[n][1] * inv, acc[n][2] * inv, acc[n][3] * inv);
+          else *reinterpret_cast<float2*>(dst) = make_float2(acc[n][0] * inv, acc[n][1] * inv);
+        }
+        if (lane == 0) s.lse[at_row] = any_key ? m[n] + log2f(l[n]) : -INFINITY;
+      }
     }
   }
+  if (beside && !final) chain_wait();           // this grid may not end before the one it runs beside
 }
 
-// one warp per row: prefix parts and own parts into the output
+// prefix parts and own parts into the output, one warp for four rows (28672 rows of two parts: 12 us, one row per warp 16)
 template <typename T, int D>
 __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ parts::Args a, const __grid_constant__ parts::Seg own,
                                                     const __grid_constant__ parts::Seg prefix, const __grid_constant__ Merge mg, int n_req) {
+  constexpr int N = 4;
   chain_release();
   chain_wait();
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int q_row[1] = {(int)(row / a.n_heads)}, head[1] = {(int)(row % a.n_heads)};
+  const int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * N;
   // rows behind the last sequence (or before the first) have no result
-  if (q_row[0] >= own.total_q || q_row[0] < own.cu_q[0] || q_row[0] >= own.cu_q[n_req]) return;
-  const bool live[1] = {true};
-  float acc[1][D / 32], m[1] = {-INFINITY}, l[1] = {0.f};
+  const int first = own.cu_q[0], last = min(own.cu_q[n_req], own.total_q);
+  int q_row[N], head[N];
+  bool live[N];
+  float acc[N][D / 32], m[N], l[N];
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) acc[0][e] = 0.f;
-  finish_rows<T, D, 1>(a, own, prefix, mg, own.first_part, own.first_part + own.splits, q_row, head, live, acc, m, l);
+  for (int n = 0; n < N; ++n) {
+    const int64_t row = min(row0 + n, own.n_rows - 1);
+    q_row[n] = (int)(row / a.n_heads);
+    head[n] = (int)(row - (int64_t)q_row[n] * a.n_heads);
+    live[n] = row0 + n < own.n_rows && q_row[n] >= first && q_row[n] < last;
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[n][e] = 0.f;
+  }
+  finish_rows<T, D, N>(a, own, prefix, mg, own.first_part, own.first_part + own.splits, q_row, head, live, acc, m, l);
 }
 
 // 32 truth values to a word: bit j of word w of a row is key 32 w + j
@@ -541,91 +555,95 @@ __global__ void __launch_bounds__(256) pack_keep_kernel(const uint8_t* __restric
 }
 
 // ------------------------------------------------------------------------------------------------ host
-struct Plan {
-  bool prefix_wide, own_wide;         // 256-row tcgen05 tiles instead of rows_kernel
-  int prefix_splits, own_splits;
+// How a segment runs.
+struct Segment {
+  bool wide;                          // 256-row tcgen05 tiles, else rows_kernel
+  int groups;                         // NG of rows_kernel
+  int64_t units;                      // CTAs in one key range each
 };
-
-// What a segment costs.  Measured on B200 (bf16, head_dim 128): 64 keys take a 256-row CTA 1.45 us (one CTA per SM) and
-// its start and end about 8 us; 64 keys take a rows_kernel CTA about 1.2 us (two per SM) and its start and end 7 us;
-// partial results are fp32, written and read back at about 4 TB/s.
-struct Cost {
-  double tile, fixed;                 // us
-  int per_sm;
-  int64_t units, tiles;               // CTAs in one range each, 64-key tiles of the longest request
-  double cta(int s) const { return fixed + tile * ((tiles + s - 1) / s); }
-  double latency(int s) const { return cta(s) * ((units * s + kNumSMs * per_sm - 1) / (kNumSMs * per_sm)); }
-  double sm_time(int s) const { return cta(s) * units * s / per_sm; }
-};
-static Cost cost_of(bool wide, int64_t requests, int64_t rows_per_request, int64_t keys, int n_kv_heads) {
-  const int64_t tile_rows = wide ? 256 : (rows_per_request <= 16 ? 16 : 32);
-  Cost c{wide ? 1.45 : 1.2, wide ? 8.0 : 7.0, wide ? 1 : 2, n_kv_heads * requests * ((rows_per_request + tile_rows - 1) / tile_rows),
-         (keys + 63) / 64};
+static Segment segment(int64_t requests, int64_t rows_per_request, int n_kv_heads) {
+  Segment c;
+  // 256-row tiles from more than 96 rows (measured: 224 rows of 32 requests 190 us in all against 227 with 32-row CTAs, a
+  // prefix part of 128 rows and 32 heads 25.5 us against 36.6, of 84 rows and 2 heads 12.1 us against 10.6)
+  c.wide = rows_per_request > 96;
+  const int64_t tile_rows = c.wide ? 256 : (rows_per_request <= 16 ? 16 : 32);
+  c.units = n_kv_heads * requests * ((rows_per_request + tile_rows - 1) / tile_rows);
+  // few CTAs: four key groups each, two CTAs per SM; many: two groups, four per SM, so that they run in fewer rounds
+  c.groups = c.units <= 2 * kNumSMs ? 4 : 2;
   return c;
 }
 
-// The two segments run beside each other: the ranges per request are chosen so that the longer of them, and the sum of
-// their work over all SMs, take the least time together with the traffic of the partial results.
-static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_len, int n_heads, int n_kv_heads, int head_dim) {
-  const int64_t g = n_heads / n_kv_heads, all = total_q * g, per_request = max_q * g;
-  const double part_us = (double)total_q * n_heads * head_dim * 8 / 4.0e6;
+struct Plan {
+  Segment pre, own;
+  int prefix_splits, own_splits;
+  bool final;                         // the own segment's CTAs merge, no merge kernel
+};
+
+// Key ranges per request.  The prefix is cut so that its CTAs fill the SMs once, into ranges of at least two tiles.  The
+// requests' own keys stay in one range, whose CTA also merges the prefix parts, unless few long ones leave most SMs idle:
+// 64 keys take a four-group CTA about 0.65 us and the merge kernel 5 us.  Measured (us): 16 requests x 32 rows x 32 heads over
+// 800 keys, own keys merged in place 66 with two prefix ranges and 69 with one, with a merge kernel 73-81; 64 tokens over
+// 32768 keys 72 with 18 ranges, 79 with a merge kernel, 83 with 14.
+static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_len, int n_heads, int n_kv_heads) {
+  const int64_t g = n_heads / n_kv_heads;
   Plan p;
-  p.prefix_wide = all > 32;
-  p.own_wide = per_request > 128;
-  const Cost pre = cost_of(p.prefix_wide, 1, all, prefix_len, n_kv_heads), own = cost_of(p.own_wide, batch, per_request, max_k, n_kv_heads);
-  double best = 1e30;
-  p.prefix_splits = p.own_splits = 1;
-  for (int so = 1; so <= 32 && (so == 1 || own.tiles / so >= 2); ++so) {
-    for (int sp = 1; sp <= 32 && (sp == 1 || pre.tiles / sp >= 2); ++sp) {
-      const double both = (pre.sm_time(sp) + own.sm_time(so)) / kNumSMs;
-      double t = fmax(both, fmax(pre.latency(sp), own.latency(so))) + (sp + so) * part_us;
-      if (so > 1 || p.own_wide) t += 4.0;          // the merge kernel
-      if (t < best * 0.98) {                       // a few per cent do not pay for more parts
-        best = t;
-        p.prefix_splits = sp;
-        p.own_splits = so;
-      }
-    }
-  }
+  p.pre = segment(1, total_q * g, n_kv_heads);
+  p.own = segment(batch, max_q * g, n_kv_heads);
+  auto splits = [](int64_t slots, int64_t units, int64_t keys, int64_t least) {
+    int64_t s = slots / units;
+    if (s > keys / least) s = keys / least;
+    return (int)(s > 32 ? 32 : (s < 1 ? 1 : s));
+  };
+  p.prefix_splits = p.pre.wide ? splits(kNumSMs, p.pre.units, prefix_len, 256) : splits(kNumSMs, p.pre.units, prefix_len, 120);
+  p.own_splits = splits(p.own.wide ? kNumSMs : 2 * kNumSMs, p.own.units, max_k, 256);
+  if (!p.own.wide && max_k / 64 * 0.65 * (p.own_splits - 1) < 5.0 * p.own_splits) p.own_splits = 1;
+  p.final = !p.own.wide && p.own_splits == 1;
   return p;
 }
 
-template <typename T, int D, int RT, bool FINAL>
+template <typename T, int D, int RT, int NG>
 static int launch_rows(const parts::Args& a, const parts::Seg& s, const parts::Seg& prefix, const Merge& mg, int n_requests,
-                       int max_q, int beside) {
-  constexpr size_t ring = (size_t)NG * NS * 2 * KB * D * 2, merge = (size_t)NG * RT * 16 * (D + 8) * 4;
-  constexpr size_t smem = RT * 16 * D * 2 + (ring > merge ? ring : merge);
-  auto kern = rows_kernel<T, D, RT, FINAL>;
+                       int max_q, int beside, int final) {
+  // with four groups two CTAs fit an SM, with two four (to the byte: 4 x (56 KB + 1 KB), head_dim 128)
+  constexpr size_t smem = (size_t)RT * 16 * D * 2 + (size_t)NG * NS * 2 * KB * D * 2;
+  auto kern = rows_kernel<T, D, RT, NG>;
   ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const int g = a.n_heads / a.n_kv_heads;
   const int64_t tiles = ((int64_t)max_q * g + RT * 16 - 1) / (RT * 16);
   if (tiles * s.splits > 65535) return ACACHE_ELIMIT;
   ACACHE_CUDA_CHECK(launch_chained(kern, dim3(a.n_kv_heads, (unsigned)(tiles * s.splits), n_requests), dim3(RT * NG * 32), smem, a.st,
-                                   a, s, prefix, mg, beside));
+                                   a, s, prefix, mg, beside, final));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;
 }
 
-template <typename T, int D, bool FINAL>
-static int launch_rows_mt(const parts::Args& a, const parts::Seg& s, const parts::Seg& prefix, const Merge& mg, int n_requests,
-                          int max_q, int beside) {
-  if ((int64_t)max_q * (a.n_heads / a.n_kv_heads) <= 16) return launch_rows<T, D, 1, FINAL>(a, s, prefix, mg, n_requests, max_q, beside);
-  return launch_rows<T, D, 2, FINAL>(a, s, prefix, mg, n_requests, max_q, beside);
+template <typename T, int D, int RT>
+static int launch_rows_ng(const parts::Args& a, const parts::Seg& s, const parts::Seg& prefix, const Merge& mg, int n_requests,
+                          int max_q, int groups, int beside, int final) {
+  if (groups == 4) return launch_rows<T, D, RT, 4>(a, s, prefix, mg, n_requests, max_q, beside, final);
+  return launch_rows<T, D, RT, 2>(a, s, prefix, mg, n_requests, max_q, beside, final);
+}
+
+// one segment: its parts (or, final, the output)
+template <typename T, int D>
+static int launch_segment(const parts::Args& a, const parts::Seg& s, const Segment& how, const parts::Seg& prefix, const Merge& mg,
+                          int n_requests, int max_q, int beside, int final) {
+  if (how.wide) return attention_wide_parts(a, s, n_requests, max_q);
+  if ((int64_t)max_q * (a.n_heads / a.n_kv_heads) <= 16)
+    return launch_rows_ng<T, D, 1>(a, s, prefix, mg, n_requests, max_q, how.groups, beside, final);
+  return launch_rows_ng<T, D, 2>(a, s, prefix, mg, n_requests, max_q, how.groups, beside, final);
 }
 
 template <typename T, int D>
-static int run(const parts::Args& a, parts::Seg prefix, parts::Seg own, Merge mg, const Plan& plan, int batch, int max_q) {
-  int rc;
+static int run(const parts::Args& a, const parts::Seg& prefix, const parts::Seg& own, const Merge& mg, const Plan& plan, int batch,
+               int max_q) {
   if (mg.n_parts > 0) {
-    rc = plan.prefix_wide ? attention_tc256_parts(a, prefix, 1, prefix.total_q)
-                          : launch_rows_mt<T, D, false>(a, prefix, prefix, mg, 1, prefix.total_q, 0);
+    const int rc = launch_segment<T, D>(a, prefix, plan.pre, prefix, mg, 1, prefix.total_q, 0, 0);
     if (rc != ACACHE_OK) return rc;
   }
-  const int beside = mg.n_parts > 0 ? 1 : 0;
-  if (!plan.own_wide && plan.own_splits == 1) return launch_rows_mt<T, D, true>(a, own, prefix, mg, batch, max_q, beside);
-  rc = plan.own_wide ? attention_tc256_parts(a, own, batch, max_q) : launch_rows_mt<T, D, false>(a, own, prefix, mg, batch, max_q, beside);
-  if (rc != ACACHE_OK) return rc;
-  ACACHE_CUDA_CHECK(launch_chained(merge_kernel<T, D>, dim3((unsigned)((own.n_rows + 3) / 4)), dim3(128), 0, a.st, a, own, prefix, mg, batch));
+  const int rc = launch_segment<T, D>(a, own, plan.own, prefix, mg, batch, max_q, mg.n_parts > 0, plan.final);
+  if (rc != ACACHE_OK || plan.final) return rc;
+  ACACHE_CUDA_CHECK(launch_chained(merge_kernel<T, D>, dim3((unsigned)((own.n_rows + 15) / 16)), dim3(128), 0, a.st, a, own, prefix, mg, batch));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;
 }
@@ -640,7 +658,7 @@ extern "C" int64_t acache_shared_prefix_attention_scratch_bytes(int total_q, int
   if (total_q <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || batch <= 0 || max_seqlen_q < 0 ||
       max_seqlen_k < 0 || prefix_len < 0)
     return 0;
-  const shared_prefix::Plan p = shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads, head_dim);
+  const shared_prefix::Plan p = shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads);
   const int64_t parts = p.prefix_splits + p.own_splits;
   return parts * total_q * n_heads * (int64_t)(head_dim + 1) * 4;
 }
@@ -669,7 +687,7 @@ extern "C" int acache_shared_prefix_attention(const void* q, int64_t q_stride, v
     return ACACHE_ELIMIT;
   if (max_seqlen_q > total_q) max_seqlen_q = total_q;
   const shared_prefix::Plan plan =
-      shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads, head_dim);
+      shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads);
   const int64_t n_rows = (int64_t)total_q * n_heads, n_parts = plan.prefix_splits + plan.own_splits;
   if (scratch_bytes < n_parts * n_rows * (head_dim + 1) * 4) return ACACHE_EINVAL;
   float* o = (float*)scratch;

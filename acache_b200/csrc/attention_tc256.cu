@@ -45,11 +45,6 @@
 // take arrivals from both; the product barriers exist in both CTAs and the commits arrive on
 // both.  No load is multicast.
 //
-// PART (shared-prefix attention, attention_shared.cu): the keys of a request are cut into part.splits
-// ranges that are CTAs of their own, a row's result stays in fp32 as (O / l, log2 of its sum) for a later
-// merge, cu_q / cu_k may be missing (one request over all query rows / over all entries of slot_map), and
-// part.keep can drop keys per row: the bits of the request that the row belongs to, two words a tile.
-//
 // O is only rescaled when a row's running maximum grows by more than 2^8 (otherwise the stale
 // reference maximum is kept; the final division by the row sum makes it exact).
 // Query-side relocation: the first shared_kv_lens[b] keys are scored against queries rotated by
@@ -58,7 +53,6 @@
 // and returns.
 #include <type_traits>
 
-#include "attention_parts.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -84,15 +78,14 @@ constexpr int RING = 8;       // tiles whose dead-key masks are kept for the row
 constexpr uint32_t kTmemCols = 512;
 constexpr int kPairRows = 1024;   // virtual rows per request from which CTA pairs are used
 
-template <typename T, typename TR, typename TC, int D, bool PAIR, bool PART>
+template <typename T, typename TR, typename TC, int D, bool PAIR>
 __global__ void __launch_bounds__(NT_ALL, 1) attention_tc256_kernel(
     const T* __restrict__ q, int64_t q_stride, T* __restrict__ out, int64_t o_stride, const T* __restrict__ k_cache,
     const T* __restrict__ v_cache, int64_t num_slots, int n_heads, int n_kv_heads, const int32_t* __restrict__ cu_q,
     const int32_t* __restrict__ cu_k, const int32_t* __restrict__ slot_map, const int32_t* __restrict__ block_tables,
     int table_stride, int block_size, float scale_log2, const int32_t* __restrict__ shared_kv_lens,
     const int32_t* __restrict__ affix_shifts, const TR* __restrict__ rope_cos, const TR* __restrict__ rope_sin,
-    int64_t rope_stride, int rope_rows, int32_t* err_flag, const __grid_constant__ parts::Seg part) {
-  static_assert(!PAIR || !PART, "the split form runs without pairs");
+    int64_t rope_stride, int rope_rows, int32_t* err_flag) {
   static_assert(!PAIR || D == 128, "a CTA of a pair stages one 64-column plane of V");
   constexpr int NC = PAIR ? 2 : 1;                // CTAs that work as one
   constexpr int CH = D * (int)sizeof(T) / 16;     // 16-byte chunks per row
@@ -124,32 +117,19 @@ __global__ void __launch_bounds__(NT_ALL, 1) attention_tc256_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = n_heads / n_kv_heads;
   const int kv_row = n_kv_heads * D;
-  const bool query_side = !PART && shared_kv_lens != nullptr && affix_shifts != nullptr;
+  const bool query_side = shared_kv_lens != nullptr && affix_shifts != nullptr;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;    // the first CTA of a pair issues its products
 
   // A pair's two CTAs are neighbours in x.  Without pairs the row tile is the slowest grid index,
   // so that the CTAs of every request's last, partly filled tile are handed out last and fill the
   // gaps of the final round instead of each delaying a full one behind it
-  const int b = PART ? blockIdx.y / part.splits : blockIdx.y, kvh = PAIR ? blockIdx.z : blockIdx.x;
+  const int b = blockIdx.y, kvh = PAIR ? blockIdx.z : blockIdx.x;
   const int tile = PAIR ? blockIdx.x : blockIdx.z, m0 = tile * (RB * BM);
   const int m0_all = PAIR ? (tile & ~1) * (RB * BM) : m0;   // first row of the pair
-  int q0, vrows, kv0, kv_len, first_tile = 0;
-  if constexpr (PART) {
-    chain_wait();          // the call's next kernel may start once every CTA is past this point,
-    chain_release();       // so that it reads nothing older kernels are still writing
-    parts::Range r = parts::request_range(part, b);
-    q0 = r.q0;
-    vrows = r.n_q * g;
-    first_tile = parts::split_range(part, (int)(blockIdx.y % part.splits), BN, r) / BN;
-    kv0 = r.k0;
-    kv_len = r.n_k;
-  } else {
-    q0 = cu_q[b];
-    vrows = (cu_q[b + 1] - q0) * g;
-    kv0 = cu_k[b];
-    kv_len = max(cu_k[b + 1] - kv0, 0);
-  }
+  const int q0 = cu_q[b];
+  const int vrows = (cu_q[b + 1] - q0) * g;
   if (m0_all >= vrows) return;
+  const int kv0 = cu_k[b], kv_len = max(cu_k[b + 1] - kv0, 0);
   int shift = 0;
   if (query_side) {
     shift = affix_shifts[b];
@@ -179,19 +159,8 @@ __global__ void __launch_bounds__(NT_ALL, 1) attention_tc256_kernel(
   const int head = kvh * g + (row_ok ? vr % g : 0);
   T* out_row = out + ((int64_t)q0 + qi) * o_stride + (int64_t)head * D;
 
-  // PART: where the row's partial result goes, and the bits of its request
-  int64_t part_row = 0;
-  const uint2* keep_words = nullptr;
-  if constexpr (PART) {
-    part_row = (int64_t)(part.first_part + blockIdx.y % part.splits) * part.n_rows + (int64_t)(q0 + qi) * n_heads + head;
-    if (part.keep && row_ok)
-      keep_words = reinterpret_cast<const uint2*>(part.keep + (int64_t)parts::request_of(part.req_cu, part.n_req, q0 + qi) * part.keep_stride) + first_tile;
-  }
-
   if (n_tiles == 0) {  // no keys: zeros
-    if constexpr (PART) {
-      if (row_ok) part.lse[part_row] = -INFINITY;
-    } else if (row_ok) {
+    if (row_ok) {
       for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(out_row + c * (16 / sizeof(T))) = make_uint4(0, 0, 0, 0);
     }
     return;
@@ -530,10 +499,6 @@ __global__ void __launch_bounds__(NT_ALL, 1) attention_tc256_kernel(
           asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(dl), "=r"(dh), "=r"(tag), "=r"(pad)
                        : "r"(dead_ring + (i % RING) * 16) : "memory");
         };
-        uint2 kept = make_uint2(0xFFFFFFFFu, 0xFFFFFFFFu);
-        if constexpr (PART) {
-          if (keep_words) kept = keep_words[i];
-        }
         read_ring();
         if (tag != (uint32_t)i + 1u) {
           const long long t0 = clock64();
@@ -544,14 +509,8 @@ __global__ void __launch_bounds__(NT_ALL, 1) attention_tc256_kernel(
           if (tag != (uint32_t)i + 1u) ok = false;
         }
         float mx = -INFINITY;
-        bool any_dead = (dl | dh) != 0u;
-        if constexpr (PART) {
-          dl |= ~kept.x;
-          dh |= ~kept.y;
-          any_dead = __any_sync(0xFFFFFFFFu, (dl | dh) != 0u);
-        }
         tmem_wait_ld();
-        if (any_dead) {   // a tile with keys that take no part (holes, the end of a run)
+        if ((dl | dh) != 0u) {   // a tile with keys that take no part (holes, the end of a run)
           const uint64_t dead = (((uint64_t)dh) << 32) | dl;
 #pragma unroll
           for (int c = 0; c < BN; ++c) {
@@ -624,24 +583,6 @@ __global__ void __launch_bounds__(NT_ALL, 1) attention_tc256_kernel(
 
     if (failed) {
       if (tid == 0 && err_flag) atomicExch(err_flag, 5);
-    } else if (PART && warp_live) {
-      // the row's partial result in fp32; a row without a live key only says so
-      const bool any_key = m_ref != -INFINITY || l_sum != 0.f;   // only NaN scores: a NaN sum
-      const float inv = any_key ? 1.0f / l_sum : 0.f;
-      uint32_t o[32];
-#pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        tmem_ld32(t_lane + col_o + c0, o);
-        tmem_wait_ld();
-        if (row_ok && any_key) {
-#pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            *reinterpret_cast<float4*>(part.o + part_row * D + c0 + c) =
-                make_float4(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv, __uint_as_float(o[c + 2]) * inv,
-                            __uint_as_float(o[c + 3]) * inv);
-        }
-      }
-      if (row_ok) part.lse[part_row] = any_key ? m_ref + log2f(l_sum) : -INFINITY;
     } else if (warp_live) {
       // thread = row: divide by the row sum and write
       const float inv = l_sum > 0.f ? 1.0f / l_sum : 0.f;
@@ -687,7 +628,7 @@ static int launch(const AttnArgs& a) {
   const int rows_per_launch_unit = NC * RB * BM;
   const int tiles = NC * ((a.max_q * g + rows_per_launch_unit - 1) / rows_per_launch_unit);
   const dim3 grid = PAIR ? dim3(tiles, a.batch, a.n_kv_heads) : dim3(a.n_kv_heads, a.batch, tiles);
-  auto kern = attention_tc256_kernel<T, TR, TC, D, PAIR, false>;
+  auto kern = attention_tc256_kernel<T, TR, TC, D, PAIR>;
   ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t lc = {};
   lc.gridDim = grid;
@@ -705,24 +646,7 @@ static int launch(const AttnArgs& a) {
       &lc, kern, (const T*)a.q, a.q_stride, (T*)a.out, a.o_stride, (const T*)a.k_cache, (const T*)a.v_cache, a.num_slots,
       a.n_heads, a.n_kv_heads, a.cu_q, a.cu_k, a.slot_map, a.block_tables, a.table_stride, a.block_size,
       a.scale * 1.4426950408889634f, a.shared_kv_lens, relocate ? a.affix_shifts : (const int32_t*)nullptr,
-      (const TR*)a.rope_cos, (const TR*)a.rope_sin, a.rope_stride, a.rope_rows, a.err_flag, parts::Seg{}));
-  ACACHE_LAUNCH_CHECK();
-  return ACACHE_OK;
-}
-
-template <typename T, int D>
-static int launch_parts(const parts::Args& a, const parts::Seg& seg, int n_requests, int max_q) {
-  constexpr size_t smem = RB * BM * D * sizeof(T) + (NSK + NSV) * BN * D * sizeof(T) + 512;
-  const int g = a.n_heads / a.n_kv_heads;
-  const int tiles = (max_q * g + RB * BM - 1) / (RB * BM);
-  auto kern = attention_tc256_kernel<T, float, float, D, false, true>;
-  ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  ACACHE_CUDA_CHECK(launch_chained(
-      kern, dim3(a.n_kv_heads, n_requests * seg.splits, tiles), dim3(NT_ALL), smem, a.st, (const T*)a.q, a.q_stride,
-      (T*)nullptr, (int64_t)0, (const T*)a.k_cache, (const T*)a.v_cache, a.num_slots, a.n_heads, a.n_kv_heads,
-      (const int32_t*)nullptr, (const int32_t*)nullptr, seg.slots, (const int32_t*)nullptr, 0, 1, a.scale_log2,
-      (const int32_t*)nullptr, (const int32_t*)nullptr, (const float*)nullptr, (const float*)nullptr, (int64_t)0, 0,
-      a.err_flag, seg));
+      (const TR*)a.rope_cos, (const TR*)a.rope_sin, a.rope_stride, a.rope_rows, a.err_flag));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;
 }
@@ -743,15 +667,6 @@ static int by_dim(const AttnArgs& a) {
 }  // namespace wide
 
 }  // namespace tc
-
-int attention_tc256_parts(const parts::Args& a, const parts::Seg& seg, int n_requests, int max_q) {
-  using namespace tc::wide;
-  if (a.dtype == ACACHE_BF16)
-    return a.head_dim == 128 ? launch_parts<__nv_bfloat16, 128>(a, seg, n_requests, max_q)
-                             : launch_parts<__nv_bfloat16, 64>(a, seg, n_requests, max_q);
-  return a.head_dim == 128 ? launch_parts<__half, 128>(a, seg, n_requests, max_q)
-                           : launch_parts<__half, 64>(a, seg, n_requests, max_q);
-}
 
 // The 256-row kernel takes requests with more than 128 virtual rows whose keys are not relocated
 // while they are staged; the caller has checked dtypes, head size, alignment and cache size.

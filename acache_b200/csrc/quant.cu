@@ -18,7 +18,7 @@
 //
 // A CTA works on a row at a time, one pass over global memory (the row stays in registers), and while it reduces
 // and rounds one row the next one it will take is on its way.  Bound by HBM at size, by latency at the few hundred rows
-// of a decode step: gate 2304 x 12288 28 us (5.0 TB/s), 512 x 12288 8.9 us; norm 4096 x 3584 16 us, 512 x 4096 3.9 us.
+// of a decode step: gate 2304 x 12288 28 us (5.0 TB/s), 512 x 12288 8.9 us; norm 4096 x 3584 14.6 us, 512 x 4096 3.3 us.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -86,8 +86,9 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return s;
 }
 
-// CTAs per SM the kernel is compiled and launched for
-constexpr int resident(int nt, int vpt) { return vpt == 1 ? 1536 / nt : (vpt == 2 ? 1280 / nt : (vpt <= 4 ? 1024 / nt : 1)); }
+// CTAs per SM the kernel is compiled and launched for: 1024 threads (1280: norm 2305 x 3584 10.1 us against 9.1; 768: gate
+// 2304 x 12288 32 us against 28), 1536 for rows of one vector a thread
+constexpr int resident(int nt, int vpt) { return vpt == 1 ? 1536 / nt : (vpt <= 4 ? 1024 / nt : 1); }
 
 template <typename T, int SRC, int NT, int VPT>
 __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const Params p) {

@@ -23,6 +23,14 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
+// true in one lane of the (converged) warp.  A branch on it tells the compiler that a single thread is active, which
+// `lane == 0` does not: tcgen05.mma takes its descriptors from uniform registers, and without that knowledge every
+// product is wrapped in a loop over the distinct values of the warp (about 150 cycles a product, whatever its size)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
 // bounded wait: false when the phase did not complete within about half a second
 constexpr long long kWaitCycles = 1000000000ll;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
