@@ -45,6 +45,13 @@ class Config:
     # other keys (16 requests, 32 heads), level with the per-request kernel over a long span (1.52
     # ms at 8192 / 3700)
     group_shared_span: bool = True
+    # block decode: multiply the shared span with the rows of all requests in one pass
+    # (``shared_prefix_attention``, instead of ``group_shared_span``) when every request reads it where it is
+    # cached; same result up to the order of the floating-point sums
+    share_span_once: bool = False
+    # run the projections of the model blocks in 8-bit integers (weights quantised per output channel at start,
+    # activations per token); changes the numbers a model computes, so it is off by default
+    int8_projections: bool = False
     # anchor selection: probe the newly admitted requests in ragged batches of at most
     # ``max_num_batched_tokens`` query rows (the reference runs one forward per request) and then
     # replay the reference's per-request allocate / free sequence on the host, so the free list,

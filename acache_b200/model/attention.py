@@ -13,7 +13,8 @@ from torch import nn
 from .. import _lib, ops
 from .._lib import check, dtype_code, ptr, stream_ptr
 from ..utils import get_context
-from .acache_attention import acache_attention, baseline_decode_attention, baseline_ragged_attention
+from .acache_attention import (acache_attention, baseline_decode_attention, baseline_ragged_attention,
+                               shared_prefix_attention)
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -79,7 +80,12 @@ class Attention(nn.Module):
                                           scale, p.importance)
         if not self.kv_already_stored:
             store_kvcache(k, v, k_cache, v_cache, ctx.slot_mapping)
-        if ctx.use_acache:
+        if ctx.shared_prefix is not None:
+            prefix_slots, keep = ctx.shared_prefix
+            o = shared_prefix_attention(q, k_cache, v_cache, prefix_slots, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
+                                        ctx.read_slot_mapping, self.scale, prefix_keep=keep,
+                                        max_seqlen_q=ctx.max_seqlen_q, max_seqlen_k=ctx.max_seqlen_k)
+        elif ctx.use_acache:
             relocating = self.shared_prefix_len > 0
             o = acache_attention(
                 q, k_cache, v_cache, ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.read_slot_mapping, self.scale,

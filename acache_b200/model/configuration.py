@@ -44,6 +44,8 @@ class LLaDAConfig:
     residual_dropout: float = 0.0
     embedding_dropout: float = 0.0
     model_type: str = "llada"
+    # long contexts: see ops.rope_frequencies ("linear", "ntk", "yarn", "llama3"); None = as trained
+    rope_scaling: dict | None = None
 
     @property
     def effective_n_kv_heads(self) -> int:
@@ -75,6 +77,7 @@ class DreamConfig:
     initializer_range: float = 0.02
     attention_dropout: float = 0.0
     model_type: str = "dream"
+    rope_scaling: dict | None = None
 
     @classmethod
     def dream_7b(cls) -> "DreamConfig":

@@ -8,14 +8,36 @@ from torch import nn
 from .. import ops
 
 
-def build_rope_table(length: int, head_dim: int, theta: float, dtype: torch.dtype, device) -> tuple[torch.Tensor, torch.Tensor]:
+def build_rope_table(length: int, head_dim: int, theta: float, dtype: torch.dtype, device,
+                     scaling: dict | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(cos, sin)`` tables ``[length, head_dim]`` in the half-split layout
     ``cat(freqs, freqs)`` (reference: nano-vdllm/model/modeling_llada.py:392-402).
-    Built once on the host in fp32 so that every device holds identical bits."""
+    Built once on the host in fp32 so that every device holds identical bits.  With ``scaling`` (a
+    model's ``rope_scaling``, see ``ops.rope_frequencies``) the angles are formed in 64 bits from the
+    stretched frequencies; an attention factor is not in the tables (``rope_score_factor``), so that
+    they stay pure rotations and cached keys can be relocated by further ones."""
+    if scaling is not None:
+        inv_freq, _ = model_rope_frequencies(head_dim, theta, scaling)
+        freqs = torch.outer(torch.arange(length, dtype=torch.float64), inv_freq)
+        emb = torch.cat((freqs, freqs), dim=-1)
+        return emb.cos().to(dtype).to(device), emb.sin().to(dtype).to(device)
     inv_freq = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float32) / head_dim))
     freqs = torch.outer(torch.arange(length, dtype=torch.float32), inv_freq)
     emb = torch.cat((freqs, freqs), dim=-1)
     return emb.cos().to(dtype).to(device), emb.sin().to(dtype).to(device)
+
+
+def model_rope_frequencies(head_dim: int, theta: float, scaling: dict):
+    """``ops.rope_frequencies`` of a served model: its tables hold for every length, so a scaling that
+    depends on the current one is refused."""
+    if scaling.get("rope_type", scaling.get("type")) == "dynamic":
+        raise ValueError("rope_type 'dynamic' changes the frequencies with the sequence length: cached keys would not fit")
+    return ops.rope_frequencies(head_dim, theta, scaling)
+
+
+def rope_score_factor(head_dim: int, theta: float, scaling: dict | None) -> float:
+    """What a scaling's attention factor (on sine and cosine of queries and keys alike) does to the scores."""
+    return 1.0 if scaling is None else model_rope_frequencies(head_dim, theta, scaling)[1] ** 2
 
 
 # Which projections of the model blocks run on this package's CTA-pair tcgen05 GEMMs
@@ -117,6 +139,40 @@ class FusedProjections:
         return self.gate_up_w
 
 
+class Int8Projections:
+    """The projections of one block in 8-bit integers (``ops.linear_int8``): copies of the weights quantised per
+    output channel, made again when the parameters were replaced; the activations are quantised per token by the
+    kernel that produces them (norm, gated activation, or ``ops.quantize_rows`` after attention)."""
+
+    def __init__(self, **projections):
+        self.projections = projections              # name -> the nn.Linear modules whose outputs lie side by side
+        for name, mods in projections.items():
+            w = mods[0].weight
+            if w.dtype not in (torch.bfloat16, torch.float16) or not w.is_cuda:
+                raise ValueError(f"8-bit projections need a 16-bit model on the GPU, not {w.dtype} on {w.device}")
+            if w.shape[1] % 16 or sum(m.weight.shape[0] for m in mods) % 16:
+                raise ValueError(f"{name}: the sizes of an 8-bit projection are multiples of 16")
+        self._made = None
+
+    def _params(self):
+        return [p for mods in self.projections.values() for m in mods for p in (m.weight, m.bias)]
+
+    def _weights(self):
+        stamp = FusedProjections._stamp_of(self._params())
+        if self._made is None or self._made[0] != stamp:
+            made = {}
+            for name, mods in self.projections.items():
+                parts = [ops.quantize_rows(m.weight.data) for m in mods]
+                bias = torch.cat([m.bias.data for m in mods]) if mods[0].bias is not None else None
+                made[name] = (torch.cat([q for q, _ in parts]), torch.cat([s for _, s in parts]), bias)
+            self._made = (stamp, made)
+        return self._made[1]
+
+    def __call__(self, name, quantised, dtype):
+        w, scale, bias = self._weights()[name]
+        return ops.linear_int8(quantised[0], quantised[1], w, scale, bias, out_dtype=dtype)
+
+
 def concat_gate_up(gate_proj, up_proj):
     """One buffer ``[2F, in]`` holding the gate rows then the up rows; the two parameters become
     views of it (state-dict names and values unchanged), so one library GEMM computes both."""
@@ -159,7 +215,13 @@ def project_qkv(h, w_qkv, b_qkv, n_heads, n_kv_heads, head_dim, position_ids, co
                                  ctx.slot_mapping)
         attn.kv_already_stored = True
         return q, None, None
-    qkv = dense(h, w_qkv, b_qkv)
+    return rotate_and_store(dense(h, w_qkv, b_qkv), n_heads, n_kv_heads, head_dim, position_ids, cos, sin, attn, ctx)
+
+
+def rotate_and_store(qkv, n_heads, n_kv_heads, head_dim, position_ids, cos, sin, attn, ctx):
+    """Splits a q/k/v projection's output, rotates q and k in place and, in a caching step, scatters k and v."""
+    n, D, nh, hkv = qkv.shape[0], head_dim, n_heads, n_kv_heads
+    caching = attn.k_cache.numel() > 0 and ctx.slot_mapping is not None
     q, k, v = qkv[:, : nh * D], qkv[:, nh * D: (nh + hkv) * D], qkv[:, (nh + hkv) * D:]
     q, k, v = q.view(n, nh, D), k.view(n, hkv, D), v.view(n, hkv, D)
     if caching:
@@ -174,15 +236,15 @@ def project_qkv(h, w_qkv, b_qkv, n_heads, n_kv_heads, head_dim, position_ids, co
 class RopeCache:
     """Grows on demand (reference: nano-vdllm/model/modeling_llada.py:373-402)."""
 
-    def __init__(self, head_dim: int, theta: float, table_dtype: torch.dtype):
-        self.head_dim, self.theta, self.table_dtype = head_dim, theta, table_dtype
+    def __init__(self, head_dim: int, theta: float, table_dtype: torch.dtype, scaling: dict | None = None):
+        self.head_dim, self.theta, self.table_dtype, self.scaling = head_dim, theta, table_dtype, scaling
         self.cos = self.sin = None
 
     def get(self, length: int, device):
         if self.cos is None or self.cos.shape[0] < length or self.cos.device != torch.device(device):
             n = max(int(length), 1)
             n = 1 << (n - 1).bit_length()  # power of two: few rebuilds
-            self.cos, self.sin = build_rope_table(n, self.head_dim, self.theta, self.table_dtype, device)
+            self.cos, self.sin = build_rope_table(n, self.head_dim, self.theta, self.table_dtype, device, self.scaling)
         return self.cos, self.sin
 
 

@@ -18,7 +18,8 @@ from ..utils import get_context
 from .attention import Attention
 from .configuration import DreamConfig
 from . import modeling_common as mc
-from .modeling_common import FusedProjections, RMSNorm, RopeCache, concat_gate_up, dense_pending, gated_mlp_input, project_qkv, select_pending
+from .modeling_common import (FusedProjections, Int8Projections, RMSNorm, RopeCache, concat_gate_up, dense_pending,
+                              gated_mlp_input, project_qkv, rope_score_factor, rotate_and_store, select_pending)
 
 
 class DreamMLP(nn.Module):
@@ -59,7 +60,9 @@ class DreamSdpaAttention(nn.Module):
         self.v_proj = nn.Linear(self.hidden_size, self.num_key_value_heads * self.head_dim, bias=True, **kw)
         self.o_proj = nn.Linear(self.num_heads * self.head_dim, self.hidden_size, bias=False, **kw)
         self.rotary_emb = rope
-        self.attn = Attention(num_heads=self.num_heads, head_dim=self.head_dim, num_kv_heads=self.num_key_value_heads)
+        factor = rope_score_factor(self.head_dim, config.rope_theta, getattr(config, "rope_scaling", None))
+        self.attn = Attention(num_heads=self.num_heads, head_dim=self.head_dim, num_kv_heads=self.num_key_value_heads,
+                              scale=None if factor == 1.0 else factor * self.head_dim ** -0.5)
         self._qkv_w = self._qkv_b = None
         self._fused = FusedProjections()
 
@@ -99,10 +102,32 @@ class DreamDecoderLayer(nn.Module):
         self.mlp = DreamMLP(config, **kw)
         self.input_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, **kw)
         self.post_attention_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, **kw)
+        self.int8 = None        # the projections in 8-bit integers, after quantize_int8()
+
+    def quantize_int8(self):
+        """Runs the layer's projections in 8-bit integers from now on."""
+        a, m = self.self_attn, self.mlp
+        self.int8 = Int8Projections(qkv=(a.q_proj, a.k_proj, a.v_proj), o=(a.o_proj,), gate_up=(m.gate_proj, m.up_proj),
+                                    down=(m.down_proj,))
+
+    def _forward_int8(self, x, position_ids, max_pos, delta):
+        a, n = self.self_attn, x.shape[0]
+        cos, sin = a.rotary_emb.get(max_pos, x.device)
+        norm = self.input_layernorm
+        qkv = self.int8("qkv", ops.rmsnorm_int8(x, norm.weight, norm.eps, delta), x.dtype)
+        q, k, v = rotate_and_store(qkv, a.num_heads, a.num_key_value_heads, a.head_dim, position_ids, cos, sin, a.attn, get_context())
+        att = a.attn(q, k, v).reshape(n, a.num_heads * a.head_dim)
+        a.attn.kv_already_stored = False
+        delta = self.int8("o", ops.quantize_rows(att), x.dtype)
+        norm = self.post_attention_layernorm
+        h = self.int8("gate_up", ops.rmsnorm_int8(x, norm.weight, norm.eps, delta), x.dtype)
+        return x, self.int8("down", ops.act_mul_halves_int8(h, self.mlp.act), x.dtype)
 
     def forward(self, x, position_ids, max_pos, delta=None):
         """Returns ``(x, delta)``: ``x`` is updated in place, the MLP output is left pending so the
         next normalisation adds it (residual add fused into the norm kernel)."""
+        if self.int8 is not None:
+            return self._forward_int8(x, position_ids, max_pos, delta)
         h = self.input_layernorm(x, delta)
         h = self.post_attention_layernorm(x, self.self_attn(h, position_ids, max_pos))
         return x, self.mlp(h)
@@ -115,7 +140,7 @@ class DreamBaseModel(nn.Module):
         self.config = config
         D = config.hidden_size // config.num_attention_heads
         # the reference casts the fp32 cos/sin to the activation dtype before use
-        self.rope = RopeCache(D, config.rope_theta, dtype or torch.float32)
+        self.rope = RopeCache(D, config.rope_theta, dtype or torch.float32, getattr(config, "rope_scaling", None))
         self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size, **kw)
         self.layers = nn.ModuleList([DreamDecoderLayer(config, i, self.rope, **kw) for i in range(config.num_hidden_layers)])
         self.norm = RMSNorm(config.hidden_size, config.rms_norm_eps, **kw)
@@ -149,6 +174,12 @@ class DreamModel(nn.Module):
                 p.fill_(1.0)
             else:
                 p.normal_(0.0, self.config.initializer_range, generator=gen)
+
+    def quantize_int8(self):
+        """See ``LLaDAModelLM.quantize_int8``."""
+        for layer in self.model.layers:
+            layer.quantize_int8()
+        return self
 
     def fuse_projections(self):
         for layer in self.model.layers:

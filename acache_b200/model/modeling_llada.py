@@ -21,7 +21,8 @@ from ..utils import get_context
 from .attention import Attention
 from .configuration import LLaDAConfig
 from . import modeling_common as mc
-from .modeling_common import FusedProjections, RMSNorm, RopeCache, concat_gate_up, dense_pending, gated_mlp_input, project_qkv, select_pending
+from .modeling_common import (FusedProjections, Int8Projections, RMSNorm, RopeCache, concat_gate_up, dense_pending,
+                              gated_mlp_input, project_qkv, rope_score_factor, rotate_and_store, select_pending)
 
 
 class LLaDALlamaBlock(nn.Module):
@@ -42,8 +43,11 @@ class LLaDALlamaBlock(nn.Module):
         self.up_proj = nn.Linear(d, ffn, bias=config.include_bias, **kw)
         self.ff_out = nn.Linear(ffn, d, bias=config.include_bias, **kw)
         self.rotary_emb = rope
-        self.attn = Attention(num_heads=config.n_heads, head_dim=d // config.n_heads,
-                              num_kv_heads=config.effective_n_kv_heads)
+        D = d // config.n_heads
+        factor = rope_score_factor(D, config.rope_theta, getattr(config, "rope_scaling", None))
+        self.attn = Attention(num_heads=config.n_heads, head_dim=D, num_kv_heads=config.effective_n_kv_heads,
+                              scale=None if factor == 1.0 else factor * D ** -0.5)
+        self.int8 = None        # the projections in 8-bit integers, after quantize_int8()
         self._qkv_w = self._qkv_b = self._gate_up_w = None
         self._fused = FusedProjections()
 
@@ -65,11 +69,30 @@ class LLaDALlamaBlock(nn.Module):
         self._gate_up_w = concat_gate_up(self.ff_proj, self.up_proj) if self.ff_proj.bias is None else None
         self._fused.reset(self._projection_params())
 
+    def quantize_int8(self):
+        """Runs the block's projections in 8-bit integers from now on."""
+        self.int8 = Int8Projections(qkv=(self.q_proj, self.k_proj, self.v_proj), attn_out=(self.attn_out,),
+                                    gate_up=(self.ff_proj, self.up_proj), ff_out=(self.ff_out,))
+
+    def _forward_int8(self, x, position_ids, max_pos, delta):
+        cfg, attn, n = self.config, self.attn, x.shape[0]
+        nh, hkv, D = cfg.n_heads, cfg.effective_n_kv_heads, cfg.d_model // cfg.n_heads
+        cos, sin = self.rotary_emb.get(max_pos, x.device)
+        qkv = self.int8("qkv", ops.rmsnorm_int8(x, self.attn_norm.weight, self.attn_norm.eps, delta), x.dtype)
+        q, k, v = rotate_and_store(qkv, nh, hkv, D, position_ids, cos, sin, attn, get_context())
+        att = attn(q, k, v).reshape(n, nh * D)
+        attn.kv_already_stored = False
+        delta = self.int8("attn_out", ops.quantize_rows(att), x.dtype)
+        h = self.int8("gate_up", ops.rmsnorm_int8(x, self.ff_norm.weight, self.ff_norm.eps, delta), x.dtype)
+        return x, self.int8("ff_out", ops.act_mul_halves_int8(h, cfg.activation_type), x.dtype)
+
     def forward(self, x: torch.Tensor, position_ids: torch.Tensor, max_pos: int, delta=None):
         """``x [n, d]`` rows of the ragged batch (updated in place), ``position_ids [n]`` int64;
         ``delta`` is the previous block's feed-forward output, still to be added to ``x``.
         Returns ``(x, delta)`` with this block's feed-forward output pending in the same way, so
         that every residual add is fused into the normalisation that follows it."""
+        if self.int8 is not None:
+            return self._forward_int8(x, position_ids, max_pos, delta)
         cfg = self.config
         n = x.shape[0]
         nh, hkv, D = cfg.n_heads, cfg.effective_n_kv_heads, cfg.d_model // cfg.n_heads
@@ -94,7 +117,7 @@ class LLaDAModel(nn.Module):
         self.config = config
         kw = dict(device=device, dtype=dtype)
         D = config.d_model // config.n_heads
-        self.rope = RopeCache(D, config.rope_theta, torch.float32)
+        self.rope = RopeCache(D, config.rope_theta, torch.float32, getattr(config, "rope_scaling", None))
         self.transformer = nn.ModuleDict(dict(
             wte=nn.Embedding(config.embedding_size or config.vocab_size, config.d_model, **kw),
             ln_f=RMSNorm(config.d_model, config.rms_norm_eps, **kw),
@@ -173,6 +196,13 @@ class LLaDAModelLM(nn.Module):
                 p.zero_()
             else:
                 p.normal_(0.0, self.config.init_std, generator=gen)
+
+    def quantize_int8(self):
+        """All blocks' projections in 8-bit integers (scales per token and output channel); the embedding and
+        the output head stay as they are.  The 16-bit parameters are kept beside the 8-bit copies."""
+        for block in self.model.transformer["blocks"]:
+            block.quantize_int8()
+        return self
 
     def fuse_projections(self):
         for block in self.model.transformer["blocks"]:

@@ -139,6 +139,11 @@ class _StaticStaging:
         return set(arrays) == set(self.offsets) and all(
             np.dtype(a.dtype) == self.offsets[k][1] and a.size <= self.offsets[k][2] for k, a in arrays.items())
 
+    def whole(self, name):
+        """The device buffer of one array at its full capacity."""
+        off, dt, n = self.offsets[name]
+        return self.dev[off: off + n * dt.itemsize].view(torch.int64 if dt == np.int64 else torch.int32)
+
     def ship(self, **arrays):
         assert self.fits(**arrays), "step metadata does not fit the captured layout"
         if self.copied is not None:
@@ -168,12 +173,12 @@ class _DecodeGraph:
     graph is replayed for every decode step with this many rows, whatever the requests are.
     ``logits`` holds what the forward returns: ``(logits, None)`` or ``(None, (x0, confidence))``."""
 
-    def __init__(self, runner, n_rows: int, names_and_dtypes: dict, read_capacity: int, max_pos: int):
+    def __init__(self, runner, n_rows: int, names_and_dtypes: dict, read_capacity: int, max_pos: int, fixed: dict | None = None):
         T = runner.config.block_length
         caps = {}
         for name, dtype in names_and_dtypes.items():
             n = {"positions": n_rows * T, "cu_q": n_rows + 1, "cu_k": n_rows + 1, "slots": n_rows * T,
-                 "read": read_capacity}.get(name, n_rows)
+                 "read": read_capacity, **(fixed or {})}.get(name, n_rows)
             caps[name] = (dtype, n)
         self.staging = _StaticStaging(runner.device, caps, runner._staging)
         self.tokens = torch.zeros(n_rows, T, dtype=torch.int64, device=runner.device)
@@ -282,6 +287,8 @@ class ModelRunner(DkvMixin):
         self._decode_graph = None
         self._graph_with_pending_timers = None
         self._rope_caches = [m.rope for m in self.model.modules() if hasattr(m, "rope") and hasattr(m.rope, "get")]
+        if getattr(config, "int8_projections", False):
+            self.base_model.quantize_int8()
         self.allocate_kv_cache()
 
     # ------------------------------------------------------------------ model access
@@ -487,7 +494,8 @@ class ModelRunner(DkvMixin):
             if cos is None:
                 theta, tdt = self._rope_spec()
                 n = 1 << max(max_position - 1, 1).bit_length()
-                cos, sin = build_rope_table(n, m.head_dim, theta, tdt, self.device)
+                cos, sin = build_rope_table(n, m.head_dim, theta, tdt, self.device,
+                                            getattr(self.config.hf_config, "rope_scaling", None))
             m.relocation_rope_cos, m.relocation_rope_sin = cos, sin
         self._affix_relocation_enabled = required
         self._affix_relocation_max_position = max_position if required else 0
@@ -512,6 +520,17 @@ class ModelRunner(DkvMixin):
         if len(spans) != 1 or next(iter(spans))[0] <= 0:
             return False
         return True
+
+    def _share_span_once(self, seqs) -> bool:
+        """Whether block decode multiplies the shared span with the rows of all requests in one pass
+        (``shared_prefix_attention``).  Needs: every request reads the same span as it is cached (no
+        relocation), a 16-bit cache and a head size the operator takes."""
+        if not getattr(self.config, "share_span_once", False) or len(seqs) < 2 or self._affix_relocation_enabled:
+            return False
+        if self.kv_cache.dtype == torch.float32 or self._arch()[2] not in (64, 128):
+            return False
+        spans = {attention_read_runs(s)[1:] for s in seqs}
+        return len(spans) == 1 and next(iter(spans))[0] > 0
 
     def _use_query_side_affix_relocation(self, relocation_materialized: bool):
         return self._affix_relocation_enabled and not relocation_materialized and self.config.max_num_seqs != 1
@@ -1071,14 +1090,15 @@ class ModelRunner(DkvMixin):
         materialized = all(getattr(s, "relocated_affix_materialized", False) for s in ps)
         use_qr = self._use_query_side_affix_relocation(materialized)
         k_lens = np.asarray([len(s) for s in ps], dtype=np.int64)
-        grouped = self._group_shared_span(ps, materialized, use_qr)
+        once = self._share_span_once(ps)
+        grouped = not once and self._group_shared_span(ps, materialized, use_qr)
         starts, slots, read, shared_lens, shifts = [], [], [], [], []
         for s in ps:
             st = s.generation_start + s.current_block_idx * T
             starts.append(st)
             slots.append(np.asarray(s.read_slot_map[st: st + T], dtype=np.int32))
-            layout, n_shared = attention_read_runs(s)[:2] if grouped else self._attention_read_layout(s, use_qr)
-            read.append(np.asarray(layout, dtype=np.int32))
+            layout, n_shared = attention_read_runs(s)[:2] if grouped or once else self._attention_read_layout(s, use_qr)
+            read.append(np.asarray(layout[n_shared:] if once else layout, dtype=np.int32))
             shared_lens.append(n_shared)
             shifts.append(s.affix_start if self._affix_relocation_enabled else 0)
         cu_k = np.zeros(len(ps) + 1, dtype=np.int32)
@@ -1086,21 +1106,31 @@ class ModelRunner(DkvMixin):
         pos = np.asarray(starts, dtype=np.int64)[:, None] + np.arange(T, dtype=np.int64)[None, :]
         arrays = dict(positions=pos, cu_q=np.arange(0, (len(ps) + 1) * T, T, dtype=np.int32), cu_k=cu_k,
                       kv_seqlens=k_lens.astype(np.int32), slots=np.concatenate(slots), read=np.concatenate(read))
-        if use_qr or grouped:
+        if once:
+            # the span as the slots it occupies, and per request a bit for every key that it reads there
+            _, span, first = attention_read_runs(ps[0])
+            keep = np.zeros((len(ps), -(-span // 64) * 64), dtype=np.uint8)
+            for i, s in enumerate(ps):
+                keep[i, :span] = attention_read_runs(s)[0][:span] >= 0
+            arrays["prefix"] = np.arange(first, first + span, dtype=np.int32)
+            arrays["keep"] = np.packbits(keep, axis=1, bitorder="little").view(np.int32)
+        elif use_qr or grouped:
             arrays["shared_lens"] = np.asarray(shared_lens, dtype=np.int32)
         if not materialized:
             arrays["shifts"] = np.asarray(shifts, dtype=np.int32)
         staging = self._staging
         self._decode_graph = None
         if graphs is not None:
-            key = (len(ps), grouped, tuple(sorted(arrays)))
+            # a shared span's length is part of the captured launches
+            key = (len(ps), grouped, arrays["prefix"].size if once else 0, tuple(sorted(arrays)))
             graph = graphs.get(key)
             if graph is None or not graph.staging.fits(**arrays):
                 # read-map capacity and RoPE table length: powers of two with head-room
                 cap = 1 << int(2 * arrays["read"].size - 1).bit_length()
                 max_pos = 1 << int(2 * int(k_lens.max()) - 1).bit_length()
                 graphs.pop(key, None)
-                graph = graphs[key] = _DecodeGraph(self, len(ps), {k: a.dtype for k, a in arrays.items()}, cap, max_pos)
+                graph = graphs[key] = _DecodeGraph(self, len(ps), {k: a.dtype for k, a in arrays.items()}, cap, max_pos,
+                                                     {k: arrays[k].size for k in ("prefix", "keep") if k in arrays})
                 self._evict_decode_graphs(graphs, keep=key)
             else:
                 graphs[key] = graphs.pop(key)      # most recently used last
@@ -1111,6 +1141,14 @@ class ModelRunner(DkvMixin):
         set_context(False, dev["cu_q"], dev["cu_k"], dev["kv_seqlens"], T, int(k_lens.max()), dev["slots"], None, True,
                     dev["read"], dev.get("shared_lens"), dev.get("shifts"))
         get_context().group_shared_span = grouped
+        if once:
+            ctx = get_context()
+            ctx.shared_prefix = (dev["prefix"], dev["keep"])
+            ctx.max_seqlen_k = int(np.diff(cu_k).max())
+            if self._decode_graph is not None:
+                # the launches that are captured serve every later step: sizes as the buffers allow, not as this step has them
+                ctx.read_slot_mapping = self._decode_graph.staging.whole("read")
+                ctx.max_seqlen_k = self._decode_graph.max_pos
         return dev["positions"]
 
     # Every captured decode forward keeps its own logits tensor ``[rows * block_length, vocab]`` alive

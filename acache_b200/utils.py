@@ -30,6 +30,9 @@ class Context:
     # not in the reference: the engine guarantees that all requests of this step name the shared
     # span the same way (see model_runner.attention_read_runs), attention may stage it per group
     group_shared_span: bool = False
+    # not in the reference: (slots of the span that all requests of this step share, keep-mask words); the read map
+    # then names each request's other keys only and attention multiplies the span once for all requests
+    shared_prefix: tuple | None = None
 
 
 _CONTEXT = Context()
