@@ -607,7 +607,8 @@ static int launch_rows(const parts::Args& a, const parts::Seg& s, const parts::S
   // with four groups two CTAs fit an SM, with two four (to the byte: 4 x (56 KB + 1 KB), head_dim 128)
   constexpr size_t smem = (size_t)RT * 16 * D * 2 + (size_t)NG * NS * 2 * KB * D * 2;
   auto kern = rows_kernel<T, D, RT, NG>;
-  ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  ACACHE_CUDA_CHECK(allow_smem((const void*)kern, smem, allowed));
   const int g = a.n_heads / a.n_kv_heads;
   const int64_t tiles = ((int64_t)max_q * g + RT * 16 - 1) / (RT * 16);
   if (tiles * s.splits > 65535) return ACACHE_ELIMIT;

@@ -449,7 +449,8 @@ static int launch(const parts::Args& a, const parts::Seg& seg, int n_requests, i
   const int g = a.n_heads / a.n_kv_heads;
   const int tiles = (max_q * g + RB * BM - 1) / (RB * BM);
   auto kern = wide_parts_kernel<T, D>;
-  ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  ACACHE_CUDA_CHECK(allow_smem((const void*)kern, smem, allowed));
   ACACHE_CUDA_CHECK(launch_chained(kern, dim3(a.n_kv_heads, n_requests * seg.splits, tiles), dim3(NT), smem, a.st, a, seg));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;

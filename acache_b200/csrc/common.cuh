@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/acache_b200.h"
 
 namespace acache {
@@ -57,6 +59,19 @@ inline cudaError_t launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block,
   lc.attrs = at;
   lc.numAttrs = chained_launches() ? 1 : 0;
   return cudaLaunchKernelEx(&lc, kern, static_cast<KArgs>(args)...);
+}
+
+// Dynamic shared memory above 48 KB has to be allowed per kernel and device; `done` (a static of the caller, one per
+// kernel and size) remembers the devices on which it was
+inline cudaError_t allow_smem(const void* kern, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // ---- element conversion ---------------------------------------------------------

@@ -118,7 +118,8 @@ template <typename T, int MT>
 static int launch_mt(const Params& p, cudaStream_t st) {
   constexpr size_t smem = (size_t)NW * MT * 16 * (COLS + 8) * 4;
   auto kern = linear_i8_few_kernel<T, MT>;
-  if (smem > 48 * 1024) ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  ACACHE_CUDA_CHECK(allow_smem((const void*)kern, smem, allowed));
   ACACHE_CUDA_CHECK(launch_chained(kern, dim3((p.N + COLS - 1) / COLS), dim3(NT), smem, st, p));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;

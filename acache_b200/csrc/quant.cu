@@ -233,7 +233,8 @@ template <typename T, int SRC, int NT, int VPT>
 static int launch_row(const Params& p, cudaStream_t st) {
   constexpr size_t smem = (size_t)(SRC == SRC_ROWS ? 1 : 2) * VPT * NT * 16;
   auto kern = quantise_kernel<T, SRC, NT, VPT>;
-  if (smem > 48 * 1024) ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  ACACHE_CUDA_CHECK(allow_smem((const void*)kern, smem, allowed));
   const int64_t most = (int64_t)kNumSMs * resident(NT, VPT);
   ACACHE_CUDA_CHECK(launch_chained(kern, dim3((unsigned)(p.n_rows < most ? p.n_rows : most)), dim3(NT), smem, st, p));
   ACACHE_LAUNCH_CHECK();

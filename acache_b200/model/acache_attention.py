@@ -197,19 +197,19 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_slots, cu_seqlens_q, cu_
     ``acache_attention`` reads the prefix once per request, its grouped form once per two requests."""
     total_q, nh, D = q.shape
     q_stride, *q_inner = q.stride()
-    dev, dtype = q.device, q.dtype
-    assert q.is_cuda and q_inner == [D, 1], "heads of a query row lie side by side"
+    dev, on, dtype = q.device, q.get_device(), q.dtype
+    assert on >= 0 and q_inner == [D, 1], "heads of a query row lie side by side"
     assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape
-    assert k_cache.dtype == dtype and v_cache.dtype == dtype and k_cache.device == dev and v_cache.device == dev
+    assert k_cache.dtype == dtype and v_cache.dtype == dtype and k_cache.get_device() == on and v_cache.get_device() == on
     hkv = k_cache.shape[-2]
     batch, P, n_slots = cu_seqlens_q.numel() - 1, prefix_slots.numel(), read_slot_mapping.numel()
     assert k_cache.shape[-1] == D and nh % hkv == 0
     for t in (prefix_slots, cu_seqlens_q, cu_seqlens_k, read_slot_mapping):
-        assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.device == dev
+        assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.get_device() == on
     assert batch >= 0 and cu_seqlens_k.numel() == batch + 1
     keep_stride = 2 * ((P + 63) // 64)
     if prefix_keep is not None:
-        assert prefix_keep.device == dev
+        assert prefix_keep.get_device() == on
         if prefix_keep.dtype == torch.bool:
             assert prefix_keep.shape == (batch, P)
             prefix_keep = pack_keep_mask(prefix_keep)

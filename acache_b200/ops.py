@@ -288,8 +288,9 @@ def linear_argmax(x: torch.Tensor, weight: torch.Tensor):
 
 # ---- projections in 8-bit integers -----------------------------------------------------------
 def _rows_of(x: torch.Tensor):
-    assert x.is_cuda and x.dim() == 2 and x.shape[1] > 0 and x.stride(1) == 1, "rows of a 2-D CUDA tensor, dense inside a row"
-    return x.shape
+    n, cols = x.shape
+    assert x.is_cuda and cols > 0 and x.stride(1) == 1, "rows of a 2-D CUDA tensor, dense inside a row"
+    return n, cols
 
 
 def _int8_rows(x, n, cols):
@@ -313,9 +314,10 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: torch
     """``quantize_rows`` of ``weight * x * rsqrt(mean(x^2) + eps)`` in one kernel, the norm kept in fp32 up to the
     rounding.  ``delta`` (optional): a residual update added to ``x`` IN PLACE first, as in ``add_rmsnorm``."""
     n, cols = _rows_of(x)
-    assert weight.shape == (cols,) and weight.dtype == x.dtype and weight.is_contiguous() and weight.device == x.device
+    assert weight.shape == (cols,) and weight.dtype == x.dtype and weight.is_contiguous() and weight.get_device() == x.get_device()
     if delta is not None:
-        assert delta.shape == x.shape and delta.dtype == x.dtype and delta.stride(1) == 1 and delta.device == x.device
+        assert delta.shape == x.shape and delta.dtype == x.dtype and delta.stride(1) == 1 and delta.get_device() == x.get_device()
+        assert n <= 1 or x.stride(0) >= cols, "rows that are updated in place may not overlap"
     q, scale = _int8_rows(x, n, cols)
     if n:
         with on_device_of(x):
@@ -342,13 +344,13 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
     """``(x int8 [n, in] @ weight int8 [out, in]^T) * x_scale[n, None] * weight_scale[None, out] (+ bias)`` with exact
     32-bit integer sums, rounded once to ``out_dtype`` (bf16 / fp16).  ``in`` and ``out`` are multiples of 16."""
     n, k = _rows_of(x)
-    N, dev = weight.shape[0], x.device
+    N, dev, on = weight.shape[0], x.device, x.get_device()
     assert x.dtype == torch.int8 and weight.dtype == torch.int8 and weight.shape == (N, k) and weight.is_contiguous()
     assert x_scale.shape == (n,) and x_scale.dtype == torch.float32 and x_scale.is_contiguous()
     assert weight_scale.shape == (N,) and weight_scale.dtype == torch.float32 and weight_scale.is_contiguous()
-    assert weight.device == dev and x_scale.device == dev and weight_scale.device == dev
+    assert weight.get_device() == on and x_scale.get_device() == on and weight_scale.get_device() == on
     if bias is not None:
-        assert bias.shape == (N,) and bias.dtype == out_dtype and bias.is_contiguous() and bias.device == dev
+        assert bias.shape == (N,) and bias.dtype == out_dtype and bias.is_contiguous() and bias.get_device() == on
     out = torch.empty(n, N, dtype=out_dtype, device=dev)
     if n:
         lib = _lib.load()
@@ -419,21 +421,21 @@ def rope_append(q, k, v, positions, inv_freq, k_cache=None, v_cache=None, slot_m
     ``(q, k)``.  ``interleaved``: pairs (2j, 2j + 1) instead of (j, j + rotary_dim / 2).  ``attention_factor``
     multiplies sine and cosine.  The table form of the half layout over the whole head is ``rope_store``."""
     n, nh, D = q.shape
-    hkv, dtype, dev = k.shape[1], q.dtype, q.device
+    hkv, dtype, dev, on = k.shape[1], q.dtype, q.device, q.get_device()
     (q_stride, *q_inner), (k_stride, *k_inner) = q.stride(), k.stride()
-    assert q.is_cuda and k.shape == (n, hkv, D) and k.dtype == dtype and k.device == dev
+    assert on >= 0 and k.shape == (n, hkv, D) and k.dtype == dtype and k.get_device() == on
     assert q_inner == [D, 1] and k_inner == [D, 1], "heads of a row lie side by side"
-    assert positions.dtype == torch.int64 and positions.shape == (n,) and positions.is_contiguous() and positions.device == dev
+    assert positions.dtype == torch.int64 and positions.shape == (n,) and positions.is_contiguous() and positions.get_device() == on
     half = inv_freq.numel()
-    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.device == dev
+    assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and inv_freq.get_device() == on
     assert 2 * half <= D, "more frequencies than pairs in a head"
     out_q = torch.empty(n, nh, D, dtype=dtype, device=dev)
     num_slots, out_k, v_stride = 0, None, 0
     if slot_mapping is not None:
         v_stride, *v_inner = v.stride()
-        assert v.shape == k.shape and v.dtype == dtype and v.device == dev and v_inner == [D, 1]
+        assert v.shape == k.shape and v.dtype == dtype and v.get_device() == on and v_inner == [D, 1]
         assert slot_mapping.dtype == torch.int32 and slot_mapping.shape == (n,) and slot_mapping.is_contiguous()
-        assert slot_mapping.device == dev and k_cache.device == dev and v_cache.device == dev
+        assert slot_mapping.get_device() == on and k_cache.get_device() == on and v_cache.get_device() == on
         assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape
         assert k_cache.dtype == dtype and v_cache.dtype == dtype and k_cache.shape[-2:] == (hkv, D)
         num_slots = k_cache.numel() // (hkv * D)
