@@ -17,6 +17,9 @@ struct Seg {
   const int32_t* keep; int64_t keep_stride;   // bits of request r: keep[r * keep_stride ...] (NULL: every key)
   const int32_t* req_cu; int n_req;           // which request a query row belongs to, for keep
   float* o; float* lse; int64_t n_rows; int first_part;   // [part][n_rows = total_q * n_heads][head_dim]
+  // 256-row tiles only: ctas > 0 shares units x unit_tiles key tiles out evenly over that many CTAs (units: KV heads x 256-row
+  // blocks of the one request); `splits` is then the number of parts that a unit may be in
+  int ctas, units, unit_tiles;
 };
 
 struct Args {

@@ -576,6 +576,7 @@ static Segment segment(int64_t requests, int64_t rows_per_request, int n_kv_head
 struct Plan {
   Segment pre, own;
   int prefix_splits, own_splits;
+  int prefix_ctas;                    // > 0: the prefix's key tiles are shared out evenly over this many CTAs
   bool final;                         // the own segment's CTAs merge, no merge kernel
 };
 
@@ -595,6 +596,18 @@ static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_l
     return (int)(s > 32 ? 32 : (s < 1 ? 1 : s));
   };
   p.prefix_splits = p.pre.wide ? splits(kNumSMs, p.pre.units, prefix_len, 256) : splits(kNumSMs, p.pre.units, prefix_len, 120);
+  p.prefix_ctas = 0;
+  if (p.pre.wide && prefix_len > 0) {
+    // rounds of whole ranges against even shares (whose CTAs start and end a range twice): 2.4 us a 128-key tile, 8 us a range
+    const int64_t tiles = (prefix_len + 127) / 128, per = (tiles + p.prefix_splits - 1) / p.prefix_splits;
+    const double ranges = (double)((p.pre.units * p.prefix_splits + kNumSMs - 1) / kNumSMs) * (per * 2.4 + 8.0);
+    const int64_t ctas = p.pre.units * tiles < kNumSMs ? p.pre.units * tiles : kNumSMs;
+    const double shares = (double)(p.pre.units * tiles) / ctas * 2.4 + 8.0 * (p.pre.units > ctas ? 1 + (p.pre.units + ctas - 1) / ctas : 2);
+    if (shares < 0.95 * ranges) {
+      p.prefix_ctas = (int)ctas;
+      p.prefix_splits = (int)((ctas + p.pre.units - 1) / p.pre.units) + 1;
+    }
+  }
   p.own_splits = splits(p.own.wide ? kNumSMs : 2 * kNumSMs, p.own.units, max_k, 256);
   if (!p.own.wide && max_k / 64 * 0.65 * (p.own_splits - 1) < 5.0 * p.own_splits) p.own_splits = 1;
   p.final = !p.own.wide && p.own_splits == 1;
@@ -696,9 +709,9 @@ extern "C" int acache_shared_prefix_attention(const void* q, int64_t q_stride, v
   const parts::Args a{q, q_stride, k_cache, v_cache, num_slots, n_heads, n_kv_heads, head_dim, dtype,
                       softmax_scale * 1.4426950408889634f, err_flag, (cudaStream_t)stream};
   const parts::Seg prefix{nullptr, nullptr, prefix_slots, prefix_len, total_q, plan.prefix_splits, prefix_keep, keep_stride, cu_seqlens_q,
-                          batch, o, lse, n_rows, 0};
+                          batch, o, lse, n_rows, 0, plan.prefix_ctas, (int)plan.pre.units, (prefix_len + 127) / 128};
   const parts::Seg own{cu_seqlens_q, cu_seqlens_k, read_slot_mapping, n_slots, total_q, plan.own_splits, nullptr, 0, nullptr, 0, o, lse,
-                       n_rows, plan.prefix_splits};
+                       n_rows, plan.prefix_splits, 0, 0, 0};
   const shared_prefix::Merge mg{out, o_stride, prefix_len > 0 ? plan.prefix_splits : 0, prefix_slots, prefix_len};
   if (dtype == ACACHE_BF16)
     return head_dim == 128 ? shared_prefix::run<__nv_bfloat16, 128>(a, prefix, own, mg, plan, batch, max_seqlen_q)

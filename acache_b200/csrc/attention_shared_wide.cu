@@ -1,7 +1,7 @@
 // Parts of shared-prefix attention (attention_shared.cu) whose rows fill the tensor cores' tiles: tcgen05 + TMEM,
 // bf16 / fp16, head_dim 64 / 128.
 //
-// One CTA = (KV head, request and key range, 256 virtual rows); a virtual row is a (query, head-of-the-GQA-group)
+// A CTA works on (KV head, request and key range, 256 virtual rows), one of them or a share of several; a virtual row is a (query, head-of-the-GQA-group)
 // pair.  The rows are two blocks of 128 that share every staged tile of 128 keys and take turns: while the tensor cores
 // work on one block's products, the other block's threads are in their softmax.  Roles hand over through mbarriers:
 //   warps 0-15   softmax: two threads per row, one for each half of a tile's keys;
@@ -51,7 +51,9 @@ constexpr uint32_t kTmemCols = 512;
 enum { BAR_K = 0, BAR_V = BAR_K + NS, BAR_S = BAR_V + NS, BAR_O = BAR_S + RB * NS, BAR_P = BAR_O + RB * NS, BAR_Q = BAR_P + RB,
        N_BARS = BAR_Q + RB };
 
-template <typename T, int D>
+// SHARES: the CTA takes a share of all tiles (s.ctas), else one part.  A template, since what a loop over pieces keeps in
+// registers costs the one-part form 3 %.
+template <typename T, int D, bool SHARES>
 __global__ void __launch_bounds__(NT, 1)
 wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__ parts::Seg s) {
   constexpr int CH = D * 2 / 16;                      // 16-byte chunks per row
@@ -74,42 +76,15 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
   auto bar = [&](int i) { return bar0 + (uint32_t)i * 8u; };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = a.n_heads / a.n_kv_heads, kvh = blockIdx.x;
-  const int b = blockIdx.y / s.splits, split = blockIdx.y % s.splits, m0 = blockIdx.z * (RB * BM);
+  const int g = a.n_heads / a.n_kv_heads;
+  // row warps: row block, TMEM lane quadrant and key half
+  const bool is_row = warp < W_ROWS;
+  const int quad = warp & 3, rb = (warp >> 2) & 1, half = warp >> 3;
+  const int row = rb * BM + quad * 32 + lane;
 
   // the call's next kernel may start once every CTA is past this point, so that it reads nothing older kernels write
   chain_wait();
   chain_release();
-  parts::Range r = parts::request_range(s, b);
-  const int vrows = r.n_q * g;
-  if (m0 >= vrows) return;
-  const int first_tile = parts::split_range(s, split, BN, r) / BN;
-  const int n_tiles = (r.n_k + BN - 1) / BN;
-
-  // row warps: row block, TMEM lane quadrant and key half
-  const bool is_row = warp < W_ROWS;
-  const int quad = warp & 3, rb = (warp >> 2) & 1, half = warp >> 3;
-  const int row = rb * BM + quad * 32 + lane, vr = m0 + row;
-  const bool row_ok = is_row && vr < vrows;
-  const int qi = row_ok ? vr / g : 0, head = kvh * g + (row_ok ? vr - qi * g : 0);
-  const int64_t part_row = (int64_t)(s.first_part + split) * s.n_rows + (int64_t)(r.q0 + qi) * a.n_heads + head;
-  if (n_tiles == 0) {
-    if (row_ok && half == 0) s.lse[part_row] = -INFINITY;
-    return;
-  }
-
-  if (tid == 0) {
-    for (int i = 0; i < 2 * NS; ++i) mbar_init(bar(BAR_K + i), 1);                    // a loader warp
-    for (int i = 0; i < 2 * RB * NS; ++i) mbar_init(bar(BAR_S + i), 1);               // product commits
-    for (int i = 0; i < 2 * RB; ++i) mbar_init(bar(BAR_P + i), 8);                    // row warps of a block
-    *give_up = 0;
-    for (int t = 0; t < RING * 2; ++t) ring_words[t * 4 + 2] = 0u;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == W_ISSUE) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
 
   auto wait_bar = [&](uint32_t at, uint32_t parity) -> bool {      // bounded; ends too when another role has given up
     const long long t0 = clock64();
@@ -137,6 +112,62 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
     __syncwarp();
     if (lane == 0) arrive(at);
   };
+
+  // One part per CTA, or (SHARES) its share of all tiles of all units, a unit being a KV head and 256 rows over the whole
+  // prefix: the share may end in the middle of a unit and go on in the next, each piece is a part.
+  [[maybe_unused]] int64_t at = 0, end = 1;
+  if constexpr (SHARES) {
+    const int64_t all = (int64_t)s.units * s.unit_tiles;
+    at = blockIdx.x * all / s.ctas;
+    end = (blockIdx.x + 1) * all / s.ctas;
+  }
+  bool first_piece = true;
+  do {
+  int kvh = blockIdx.x, m0 = blockIdx.z * (RB * BM), part, first_tile, spare = 0;
+  parts::Range r = parts::request_range(s, SHARES ? 0 : blockIdx.y / s.splits);
+  const int vrows = r.n_q * g;
+  if constexpr (SHARES) {
+    const int64_t all = (int64_t)s.units * s.unit_tiles;
+    const int unit = (int)(at / s.unit_tiles);
+    const int64_t unit0 = (int64_t)unit * s.unit_tiles;
+    first_tile = (int)(at - unit0);
+    const int last_tile = (int)min((int64_t)s.unit_tiles, end - unit0);
+    kvh = unit % a.n_kv_heads;
+    m0 = unit / a.n_kv_heads * (RB * BM);
+    part = (int)(blockIdx.x - ((unit0 + 1) * s.ctas - 1) / all);        // CTAs since the one that holds the unit's first tile
+    if (last_tile == s.unit_tiles) spare = s.splits - 1 - part;         // parts of the unit that no CTA has
+    r.k0 += first_tile * BN;
+    r.n_k = min(r.n_k, last_tile * BN) - first_tile * BN;
+    at = unit0 + last_tile;
+  } else {
+    part = blockIdx.y % s.splits;
+    if (m0 >= vrows) return;
+    first_tile = parts::split_range(s, part, BN, r) / BN;
+  }
+  const int n_tiles = (r.n_k + BN - 1) / BN;
+  const int vr = m0 + row;
+  const bool row_ok = is_row && vr < vrows;
+  const int qi = row_ok ? vr / g : 0, head = kvh * g + (row_ok ? vr - qi * g : 0);
+  const int64_t part_row = (int64_t)(s.first_part + part) * s.n_rows + (int64_t)(r.q0 + qi) * a.n_heads + head;
+  if (n_tiles == 0) {                                  // not with shares: a share has a tile of every unit it touches
+    if (row_ok && half == 0) s.lse[part_row] = -INFINITY;
+    return;
+  }
+
+  if (tid == 0) {
+    if (!first_piece)
+      for (int i = 0; i < N_BARS; ++i) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar(i)) : "memory");
+    for (int i = 0; i < 2 * NS; ++i) mbar_init(bar(BAR_K + i), 1);                    // a loader warp
+    for (int i = 0; i < 2 * RB * NS; ++i) mbar_init(bar(BAR_S + i), 1);               // product commits
+    for (int i = 0; i < 2 * RB; ++i) mbar_init(bar(BAR_P + i), 8);                    // row warps of a block
+    if (first_piece) *give_up = 0;
+    for (int t = 0; t < RING * 2; ++t) ring_words[t * 4 + 2] = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (first_piece && warp == W_ISSUE) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
 
   // ---- the queries, while TMEM is being allocated
   if (is_row) {
@@ -433,27 +464,39 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
         }
         __syncwarp();
       }
-      if (row_ok && half == 0) s.lse[part_row] = any_key ? m_ref + log2f(l_sum) : -INFINITY;
+      if (row_ok && half == 0) {
+        s.lse[part_row] = any_key ? m_ref + log2f(l_sum) : -INFINITY;
+        for (int i = 1; i <= spare; ++i) s.lse[part_row + i * s.n_rows] = -INFINITY;
+      }
     }
   }
   cp_async_wait<0>();
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(*give_up)) break;
+  tc_fence_after();
+  first_piece = false;
+  } while (SHARES && at < end);
   if (warp == W_ISSUE)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(kTmemCols) : "memory");
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SHARES>
 static int launch(const parts::Args& a, const parts::Seg& seg, int n_requests, int max_q) {
   constexpr size_t smem = (size_t)RB * BM * D * 2 + (size_t)2 * NS * BN * D * 2 + N_BARS * 8 + 16 + RING * 32 + 16 + 2 * 256 * 4;
   const int g = a.n_heads / a.n_kv_heads;
   const int tiles = (max_q * g + RB * BM - 1) / (RB * BM);
-  auto kern = wide_parts_kernel<T, D>;
+  auto kern = wide_parts_kernel<T, D, SHARES>;
   static std::atomic<uint64_t> allowed{0};
   ACACHE_CUDA_CHECK(allow_smem((const void*)kern, smem, allowed));
-  ACACHE_CUDA_CHECK(launch_chained(kern, dim3(a.n_kv_heads, n_requests * seg.splits, tiles), dim3(NT), smem, a.st, a, seg));
+  const dim3 grid = SHARES ? dim3(seg.ctas) : dim3(a.n_kv_heads, n_requests * seg.splits, tiles);
+  ACACHE_CUDA_CHECK(launch_chained(kern, grid, dim3(NT), smem, a.st, a, seg));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;
+}
+
+template <typename T, int D>
+static int launch_form(const parts::Args& a, const parts::Seg& seg, int n_requests, int max_q) {
+  return seg.ctas > 0 ? launch<T, D, true>(a, seg, n_requests, max_q) : launch<T, D, false>(a, seg, n_requests, max_q);
 }
 
 }  // namespace wide_parts
@@ -461,8 +504,8 @@ static int launch(const parts::Args& a, const parts::Seg& seg, int n_requests, i
 int attention_wide_parts(const parts::Args& a, const parts::Seg& seg, int n_requests, int max_q) {
   using namespace wide_parts;
   if (a.dtype == ACACHE_BF16)
-    return a.head_dim == 128 ? launch<__nv_bfloat16, 128>(a, seg, n_requests, max_q) : launch<__nv_bfloat16, 64>(a, seg, n_requests, max_q);
-  return a.head_dim == 128 ? launch<__half, 128>(a, seg, n_requests, max_q) : launch<__half, 64>(a, seg, n_requests, max_q);
+    return a.head_dim == 128 ? launch_form<__nv_bfloat16, 128>(a, seg, n_requests, max_q) : launch_form<__nv_bfloat16, 64>(a, seg, n_requests, max_q);
+  return a.head_dim == 128 ? launch_form<__half, 128>(a, seg, n_requests, max_q) : launch_form<__half, 64>(a, seg, n_requests, max_q);
 }
 
 }  // namespace acache

@@ -255,3 +255,27 @@ def test_bad_slots_are_reported_and_refusals():
             _run(m, *args)
     with pytest.raises(AssertionError):
         _run(m, *case[:7], torch.ones(2, 69, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("q_lens,nh,hkv,D,prefix,drop", [([100] * 13, 4, 2, 128, 12800, 0.0), ([700, 1, 659, 80], 6, 2, 64, 16000, 0.3),
+                                                        ([40] * 128, 8, 1, 128, 3000, 0.1)])
+def test_prefix_tiles_shared_out_over_all_sms(q_lens, nh, hkv, D, prefix, drop):
+    """Row blocks that do not divide the SMs evenly: a CTA's share ends inside one row block's keys and goes on in the
+    next (20, 17 x 2 and 160 blocks of 256 rows over 100, 125 and 24 key tiles)."""
+    _lib, m = _fn()
+    k_lens = [3 + i % 5 for i in range(len(q_lens))]
+    q, kc, vc, pre, cu_q, cu_k, slots, keep = _inputs(q_lens, k_lens, prefix, nh, hkv, D, BF, seed=2, drop=drop)
+    got = _run(m, q, kc, vc, pre, cu_q, cu_k, slots, keep).cpu().double()
+    again = _run(m, q, kc, vc, pre, cu_q, cu_k, slots, keep).cpu().double()
+    assert torch.equal(got, again)
+    g = torch.Generator().manual_seed(1)
+    K, V = kc.to(DEV).view(-1, hkv, D), vc.to(DEV).view(-1, hkv, D)
+    for b in sorted({0, 1, len(q_lens) - 1, len(q_lens) // 2}):
+        p = pre if keep is None else pre[keep[b]]
+        names = torch.cat([p, slots[cu_k[b]:cu_k[b + 1]]]).long().to(DEV)
+        for h in range(nh):
+            k, v = K[names, h * hkv // nh].double(), V[names, h * hkv // nh].double()
+            w = torch.softmax((q[cu_q[b]:cu_q[b + 1], h].to(DEV).double() @ k.T) * D ** -0.5, -1)
+            ref, size = (w @ v).cpu(), (w @ v.abs()).cpu()
+            assert ((got[cu_q[b]:cu_q[b + 1], h] - ref).abs() <= _tolerance(ref, size, BF)).all()
+    _lib.check_device_errors()
