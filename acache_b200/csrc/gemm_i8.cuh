@@ -6,11 +6,12 @@
 namespace acache {
 namespace few {
 
-// Measured on B200 against 256-row tiles with K slices (us): 16 rows: 4096 x 4096 5.5 against 9.5, 4096 x 12288 17.7
-// against 19.1, 12288 x 4096 15.4 against 16.1, 3584 x 37888 42.7 against 35.6; 33 rows: 4096 x 4096 9.1 against 10.2,
-// 4096 x 12288 29 against 18.5, 12288 x 4096 28 against 17; 64 rows: 4096 x 4096 9.9 against 11.6.
+// Measured on B200 against 256-row tiles with K slices (us): 16 rows: 4096 x 4096 4.3 against 9.3, 4096 x 12288 13.5
+// against 20.0, 12288 x 4096 11.4 against 15.8, 3584 x 37888 about 36 either way; 32 rows: 4096 x 4096 5.5 against 9.8,
+// 4096 x 12288 16.0 against 18.3, 12288 x 4096 13.3 against 16.6, 3584 x 18944 21.0 against 20.2; 33 rows: 4096 x 4096
+// 7.9 against 9.9, 4096 x 12288 29 against 18.1, 12288 x 4096 28 against 16.6.
 inline bool takes(int rows, int out_features, int in_features) {
-  if (rows <= 16) return out_features <= 24576;
+  if (rows <= 32) return out_features <= 24576;
   return rows <= 64 && out_features <= 32 * 148 && in_features <= 6144;      // one CTA per SM
 }
 

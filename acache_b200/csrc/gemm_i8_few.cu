@@ -3,13 +3,13 @@
 //
 //   out[i, j] = (sum_k x[i, k] w[j, k]) * x_scale[i] * w_scale[j] (+ bias[j]),   sums exact in 32-bit integers
 //
-// A CTA owns 32 columns and all rows; its eight warps split the K range in steps of 64 and are added through shared
+// A CTA owns 32 columns and all rows; its 8 or 16 warps split the K range in steps of 64 and are added through shared
 // memory at the end.  The operands go from global memory straight into the fragments of the m16n8k32 integer
 // products: which k an element belongs to does not matter as long as both operands agree, so the four lanes that
 // share a row each load 16 consecutive bytes of its 64 and feed them to two products as (bytes 0-7) and (bytes 8-15).
 // No staging, no barrier before the end, and one launch (a pair of CTAs on 256-row tcgen05 tiles takes 15 us for 33 x
 // 4096 x 4096 whatever its tile, since one 128-byte k block costs it 0.39 us, and 10 us in 4 K slices with a second launch
-// that adds them; this kernel 9 us, and 5 us for one row: 3.4 TB/s of weights).  gemm_i8.cuh has the rule.
+// that adds them; this kernel 8 us, and 4 us for one row: 4.3 TB/s of weights).  gemm_i8.cuh has the rule.
 #include "gemm_i8.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -17,7 +17,10 @@
 namespace acache {
 namespace few {
 
-constexpr int NW = 8, NT = NW * 32, COLS = 32, NB = COLS / 8;
+constexpr int COLS = 32, NB = COLS / 8;
+// warps of a CTA: 16 for up to 32 rows (16 x 12288 x 4096: 11.4 us against 13.7 with 8), 8 where the registers allow no
+// more.  The kernel is compiled for one CTA per SM: left to itself the compiler keeps fewer loads in flight (24 us)
+template <int MT> constexpr int kWarps = MT <= 2 ? 16 : 8;
 
 __device__ __forceinline__ void mma_i8(int32_t* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -25,7 +28,8 @@ __device__ __forceinline__ void mma_i8(int32_t* c, uint32_t a0, uint32_t a1, uin
 }
 
 template <typename T, int MT>
-__global__ void __launch_bounds__(NT) linear_i8_few_kernel(const Params p) {
+__global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_i8_few_kernel(const Params p) {
+  constexpr int NW = kWarps<MT>, NT = NW * 32;
   chain_release();
   chain_wait();
   constexpr int LD = COLS + 8;                        // rows 8 banks apart: a half warp's 64-bit stores do not collide
@@ -53,7 +57,7 @@ __global__ void __launch_bounds__(NT) linear_i8_few_kernel(const Params p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][n][e] = 0;
 
-  constexpr int DEPTH = MT == 1 ? 4 : (MT == 2 ? 3 : 2);     // steps in flight, as the registers allow
+  constexpr int DEPTH = 2;                            // steps in flight per warp
   uint4 a[DEPTH][2 * MT], b[DEPTH][NB];
   auto load = [&](int buf, int k0) {
     const int k = k0 + kq;
@@ -116,11 +120,11 @@ __global__ void __launch_bounds__(NT) linear_i8_few_kernel(const Params p) {
 
 template <typename T, int MT>
 static int launch_mt(const Params& p, cudaStream_t st) {
-  constexpr size_t smem = (size_t)NW * MT * 16 * (COLS + 8) * 4;
+  constexpr size_t smem = (size_t)kWarps<MT> * MT * 16 * (COLS + 8) * 4;
   auto kern = linear_i8_few_kernel<T, MT>;
   static std::atomic<uint64_t> allowed{0};
   ACACHE_CUDA_CHECK(allow_smem((const void*)kern, smem, allowed));
-  ACACHE_CUDA_CHECK(launch_chained(kern, dim3((p.N + COLS - 1) / COLS), dim3(NT), smem, st, p));
+  ACACHE_CUDA_CHECK(launch_chained(kern, dim3((p.N + COLS - 1) / COLS), dim3(kWarps<MT> * 32), smem, st, p));
   ACACHE_LAUNCH_CHECK();
   return ACACHE_OK;
 }

@@ -253,3 +253,67 @@ def test_rope_append_reports_slots_outside_the_cache():
         _lib.check_device_errors()
     written = (vc.view(256, -1).abs().sum(1) > 0).nonzero().flatten().tolist()
     assert written == [3]
+
+
+def test_offsets_beyond_32_bits():
+    """Outputs, weights and cache rows whose element offsets pass 2^31."""
+    _lib, ops = _ops()
+    g = torch.Generator().manual_seed(0)
+    n, out, k = 17000, 126464, 16                     # 2.15e9 outputs
+    x = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8).to(DEV)
+    w = torch.randint(-128, 128, (out, k), generator=g, dtype=torch.int8).to(DEV)
+    xs, ws = torch.rand(n, generator=g).to(DEV), torch.rand(out, generator=g).to(DEV)
+    y = ops.linear_int8(x, xs, w, ws)
+    for rows in (slice(0, 3), slice(n - 300, n)):
+        ref = (x[rows].double() @ w.double().T) * xs[rows].double()[:, None] * ws.double()
+        assert ((y[rows].double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -21)).all()
+    del y
+    w = torch.randint(-128, 128, (131056, 16512), dtype=torch.int8, device=DEV)      # 2.16e9 weights
+    ws = torch.rand(131056, device=DEV)
+    x = torch.randint(-128, 128, (40, 16512), dtype=torch.int8, device=DEV)
+    y = ops.linear_int8(x, xs[:40], w, ws)
+    ref = (x.double() @ w[-64:].double().T) * xs[:40].double()[:, None] * ws[-64:].double()
+    assert ((y[:, -64:].double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -21)).all()
+    del w, y
+    big = torch.zeros(2, 2 ** 30 + 64, dtype=torch.float16, device=DEV)[:, :4096]    # rows 2^30 elements apart
+    big[1] = torch.randn(4096, device=DEV).half()
+    q, _ = ops.quantize_rows(big)
+    assert torch.equal(q.double(), _quantise64(big.double())[0])
+    del big
+    pages = 2 ** 31 // (256 * 32 * 128) + 2
+    kc = torch.empty(pages, 256, 32, 128, dtype=BF, device=DEV)
+    vc = torch.empty_like(kc)
+    t = torch.randn(6, 32, 128, device=DEV).to(BF)
+    slots = torch.arange(pages * 256 - 6, pages * 256, dtype=torch.int32, device=DEV)
+    inv = ops.rope_frequencies(128, 500000.0)[0].to(DEV)
+    ops.rope_append(t, t, t, torch.arange(6, device=DEV), inv, kc, vc, slots)
+    assert torch.equal(vc.view(-1, 32, 128)[-6:], t)
+    _close_rotated(kc.view(-1, 32, 128)[-6:], _rotate64(t.cpu(), torch.arange(6), inv, False, 1.0), t)
+    _lib.check_device_errors()
+
+
+def test_rmsnorm_int8_refuses_rows_that_overlap_when_it_writes_them():
+    _lib, ops = _ops()
+    x = torch.randn(1, 64, device=DEV).to(BF)
+    w = torch.ones(64, dtype=BF, device=DEV)
+    q, s = ops.rmsnorm_int8(x.expand(4, 64), w, 1e-5)            # read only: fine
+    assert torch.equal(q[0], q[3])
+    with pytest.raises(AssertionError):
+        ops.rmsnorm_int8(x.expand(4, 64), w, 1e-5, torch.zeros(4, 64, dtype=BF, device=DEV))
+
+
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 31, 32, 33, 48, 49, 64, 65, 255, 256, 257])
+@pytest.mark.parametrize("k,out", [(16, 32), (80, 48), (1040, 4112), (4096, 1008)])
+def test_linear_int8_at_the_edges_of_its_forms(n, k, out):
+    """Row counts around the few-row kernel's tiles and the 256-row ones, K ranges that end inside a step of 64 or a
+    k block of 128, column counts that end inside a tile; rows of a wider tensor; integers, so every sum is exact."""
+    _lib, ops = _ops()
+    g = torch.Generator().manual_seed(n * k)
+    wide = torch.randint(-128, 128, (n, k + 32), generator=g, dtype=torch.int8).to(DEV)
+    x = wide[:, 16:16 + k]
+    w = torch.randint(-128, 128, (out, k), generator=g, dtype=torch.int8).to(DEV)
+    xs, ws = torch.rand(n, generator=g).to(DEV), torch.rand(out, generator=g).to(DEV)
+    y = ops.linear_int8(x, xs, w, ws)
+    ref = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
+    assert ((y.double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -21)).all()
+    _lib.check_device_errors()

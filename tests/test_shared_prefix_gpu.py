@@ -279,3 +279,49 @@ def test_prefix_tiles_shared_out_over_all_sms(q_lens, nh, hkv, D, prefix, drop):
             ref, size = (w @ v).cpu(), (w @ v.abs()).cpu()
             assert ((got[cu_q[b]:cu_q[b + 1], h] - ref).abs() <= _tolerance(ref, size, BF)).all()
     _lib.check_device_errors()
+
+
+def test_slots_beyond_32_bit_offsets_and_the_largest_batch():
+    """Cache rows whose element offsets pass 2^31, and 2047 requests in one call (one more is refused)."""
+    _lib, m = _fn()
+    nh = hkv = 32
+    D, page = 128, 256
+    pages = 2 ** 31 // (page * hkv * D) + 8             # 2048 pages and a few: offsets above 2^31 elements
+    kc = torch.empty(pages, page, hkv, D, dtype=BF, device=DEV)
+    vc = torch.empty_like(kc)
+    g = torch.Generator().manual_seed(0)
+    last = (pages - 4) * page
+    k_new, v_new = torch.randn(4 * page, hkv, D, generator=g).to(BF), torch.randn(4 * page, hkv, D, generator=g).to(BF)
+    kc.view(-1, hkv, D)[last:], vc.view(-1, hkv, D)[last:] = k_new.to(DEV), v_new.to(DEV)
+    for q_lens in ([1, 1], [1, 40], [5, 130]):
+        q = torch.randn(sum(q_lens), nh, D, generator=g).to(BF)
+        pre = torch.arange(300, dtype=torch.int32)
+        own = torch.arange(400, 640, dtype=torch.int32)
+        cu_q = torch.tensor([0, q_lens[0], sum(q_lens)], dtype=torch.int32)
+        cu_k = torch.tensor([0, 100, 240], dtype=torch.int32)
+        got = m.shared_prefix_attention(q.to(DEV), kc, vc, (pre + last).to(DEV), cu_q.to(DEV), cu_k.to(DEV), (own + last).to(DEV)).cpu().double()
+        ref, size = _reference(q, k_new.view(4, page, hkv, D), v_new.view(4, page, hkv, D), pre, cu_q.tolist(), cu_k.tolist(), own, D ** -0.5)
+        assert ((got - ref).abs() <= _tolerance(ref, size, BF)).all()
+    del kc, vc
+    n = 2047
+    q, kc, vc, pre, cu_q, cu_k, slots, keep = _inputs([1] * n, [i % 3 for i in range(n)], 70, 2, 1, 64, BF, drop=0.5)
+    _check(m, (q, kc, vc, pre, cu_q, cu_k, slots, keep))
+    with pytest.raises(OverflowError):
+        _run(m, torch.cat([q, q[:1]]), kc, vc, pre, torch.arange(n + 2, dtype=torch.int32), torch.cat([cu_k, cu_k[-1:]]), slots, None)
+    _lib.check_device_errors()
+
+
+def test_bad_offsets_stay_inside_the_arrays():
+    """Offsets that run backwards or past the arrays: nothing outside is read or written, the other rows are right."""
+    _lib, m = _fn()
+    for q_lens in ([2, 3, 2], [40, 60, 70]):
+        q, kc, vc, pre, cu_q, cu_k, slots, _ = _inputs(q_lens, [10, 20, 30], 150, 4, 2, 64, BF)
+        want = _run(m, q, kc, vc, pre, cu_q, cu_k, slots, None, max_seqlen_q=max(q_lens), max_seqlen_k=30)
+        bad_q, bad_k = cu_q.clone(), cu_k.clone()
+        bad_q[-1] = 10 ** 6
+        bad_k[-1] = 10 ** 6
+        got = _run(m, q, kc, vc, pre, bad_q, bad_k, slots, None, max_seqlen_q=max(q_lens), max_seqlen_k=30)
+        assert torch.equal(got, want)
+        bad_k[1] = -5
+        got = _run(m, q, kc, vc, pre, cu_q, bad_k, slots, None, max_seqlen_q=max(q_lens), max_seqlen_k=30)
+        assert torch.isfinite(got).all() and torch.equal(got[cu_q[2]:], want[cu_q[2]:])
