@@ -120,10 +120,10 @@ __device__ __noinline__ void recompute_prefix(const parts::Args& a, const parts:
 
 // one warp: parts [begin, end) of N rows added to (acc, m, l), acc = the sum of weights 2^(score - m) times V.
 // The loads of the N rows, and of several parts, are in flight together.
-template <int D, int N>
+template <int D, int N, int U>
 __device__ __forceinline__ void merge_parts(const parts::Seg& s, int begin, int end, const int64_t (&row)[N], const bool (&live)[N],
                                             float (&acc)[N][D / 32], float (&m)[N], float (&l)[N]) {
-  constexpr int E = D / 32, U = N == 1 ? 4 : 2;      // parts whose loads are in flight together
+  constexpr int E = D / 32;                          // U: parts whose loads are in flight together
   const int lane = threadIdx.x & 31;
   for (int base = begin; base < end; base += 32) {
     const int cnt = min(32, end - base);
@@ -188,8 +188,8 @@ __device__ __noinline__ void finish_again(const parts::Args& a, const parts::Seg
     own[0][e] = own_acc[e];
     pre[0][e] = 0.f;
   }
-  merge_parts<D, 1>(s, own_begin, own_end, row, live, own, m, l);
-  merge_parts<D, 1>(s, 0, mg.n_parts, row, live, pre, pm, pl);
+  merge_parts<D, 1, 4>(s, own_begin, own_end, row, live, own, m, l);
+  merge_parts<D, 1, 4>(s, 0, mg.n_parts, row, live, pre, pm, pl);
   if (pl[0] > 0.f) {
     float again[E];
     recompute_prefix<T, D>(a, prefix, mg, q_row, head, pm[0] + log2f(pl[0]), again);
@@ -206,7 +206,7 @@ __device__ __noinline__ void finish_again(const parts::Args& a, const parts::Seg
 
 // one warp: the final values of N rows from (acc, m, l) of the keys that have no part in the workspace, the prefix
 // parts and own parts [own_begin, own_end)
-template <typename T, int D, int N>
+template <typename T, int D, int N, int U>
 __device__ __forceinline__ void finish_rows(const parts::Args& a, const parts::Seg& s, const parts::Seg& prefix, const Merge& mg,
                                             int own_begin, int own_end, const int (&q_row)[N], const int (&head)[N],
                                             const bool (&live)[N], float (&acc)[N][D / 32], float (&m)[N], float (&l)[N]) {
@@ -223,7 +223,7 @@ __device__ __forceinline__ void finish_rows(const parts::Args& a, const parts::S
     for (int e = 0; e < E; ++e) acc0[n][e] = acc[n][e];
   }
   // the prefix's parts and the own ones follow each other in the workspace
-  merge_parts<D, N>(s, mg.n_parts > 0 ? 0 : own_begin, mg.n_parts > 0 && own_end == own_begin ? mg.n_parts : own_end, row, live, acc, m, l);
+  merge_parts<D, N, U>(s, mg.n_parts > 0 ? 0 : own_begin, mg.n_parts > 0 && own_end == own_begin ? mg.n_parts : own_end, row, live, acc, m, l);
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     if (!live[n]) continue;
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(RT * NG * 32, 8 / NG) rows_kernel(const __grid
       }
     }
     if (final) {
-      finish_rows<T, D, N>(a, s, prefix, mg, s.first_part, s.first_part, q_row, head, live, acc, m, l);
+      finish_rows<T, D, N, RT == 1 ? 6 : 2>(a, s, prefix, mg, s.first_part, s.first_part, q_row, head, live, acc, m, l);
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ part
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) acc[n][e] = 0.f;
   }
-  finish_rows<T, D, N>(a, own, prefix, mg, own.first_part, own.first_part + own.splits, q_row, head, live, acc, m, l);
+  finish_rows<T, D, N, 2>(a, own, prefix, mg, own.first_part, own.first_part + own.splits, q_row, head, live, acc, m, l);
 }
 
 // 32 truth values to a word: bit j of word w of a row is key 32 w + j
@@ -587,6 +587,7 @@ struct Plan {
 // 32768 keys 72 with 18 ranges, 79 with a merge kernel, 83 with 14.
 static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_len, int n_heads, int n_kv_heads) {
   const int64_t g = n_heads / n_kv_heads;
+  if (max_q > total_q) max_q = total_q;
   Plan p;
   p.pre = segment(1, total_q * g, n_kv_heads);
   p.own = segment(batch, max_q * g, n_kv_heads);
@@ -598,11 +599,13 @@ static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_l
   p.prefix_splits = p.pre.wide ? splits(kNumSMs, p.pre.units, prefix_len, 256) : splits(kNumSMs, p.pre.units, prefix_len, 120);
   p.prefix_ctas = 0;
   if (p.pre.wide && prefix_len > 0) {
-    // rounds of whole ranges against even shares (whose CTAs start and end a range twice): 2.4 us a 128-key tile, 8 us a range
+    // rounds of whole ranges against even shares (whose CTAs start and end a range twice): 2.4 us a 128-key tile, 8 us a range,
+    // 0.3 us for every part that a row's merge reads
     const int64_t tiles = (prefix_len + 127) / 128, per = (tiles + p.prefix_splits - 1) / p.prefix_splits;
-    const double ranges = (double)((p.pre.units * p.prefix_splits + kNumSMs - 1) / kNumSMs) * (per * 2.4 + 8.0);
+    const double ranges = (double)((p.pre.units * p.prefix_splits + kNumSMs - 1) / kNumSMs) * (per * 2.4 + 8.0) + 0.3 * p.prefix_splits;
     const int64_t ctas = p.pre.units * tiles < kNumSMs ? p.pre.units * tiles : kNumSMs;
-    const double shares = (double)(p.pre.units * tiles) / ctas * 2.4 + 8.0 * (p.pre.units > ctas ? 1 + (p.pre.units + ctas - 1) / ctas : 2);
+    const double shares = (double)(p.pre.units * tiles) / ctas * 2.4 + 8.0 * (p.pre.units > ctas ? 1 + (p.pre.units + ctas - 1) / ctas : 2) +
+                          0.3 * ((ctas + p.pre.units - 1) / p.pre.units + 1);
     if (shares < 0.95 * ranges) {
       p.prefix_ctas = (int)ctas;
       p.prefix_splits = (int)((ctas + p.pre.units - 1) / p.pre.units) + 1;
@@ -699,7 +702,7 @@ extern "C" int acache_shared_prefix_attention(const void* q, int64_t q_stride, v
   if (num_slots > 0x7FFFFFFFll || batch > 65535 / 32 || prefix_len > (1 << 30) || n_slots > (1 << 30) ||
       (int64_t)total_q * (n_heads / n_kv_heads) > (1 << 23) || n_kv_heads > 65535)
     return ACACHE_ELIMIT;
-  if (max_seqlen_q > total_q) max_seqlen_q = total_q;
+  if (max_seqlen_q > total_q) max_seqlen_q = total_q;     // as the plan takes it
   const shared_prefix::Plan plan =
       shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads);
   const int64_t n_rows = (int64_t)total_q * n_heads, n_parts = plan.prefix_splits + plan.own_splits;
