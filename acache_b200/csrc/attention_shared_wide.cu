@@ -378,7 +378,8 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
             out[c / 2] = pack2<T>(p0, p1);
           }
         };
-        auto weigh_all = [&]() {                       // xa is on its way
+        bool leave = false;
+        for (;;) {                                     // xa is on its way
           const float m_use = m_ref == -INFINITY ? 0.f : m_ref;    // no live key so far: every weight is 0 (or not used)
           const uint64_t nm2 = pack_f32x2(-m_use, -m_use);
           rs2 = pack_f32x2(0.f, 0.f);
@@ -388,14 +389,12 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
           weigh(xa, dl, w, nm2);
           tmem_wait_ld();
           weigh(xb, dh, w + 16, nm2);
-        };
-        weigh_all();
-        mx *= a.scale_log2;
-        // does any of the 64 threads see a score beyond its row's reference (or know of a wait that ran out)?
-        if (vote(mx > m_ref + 8.0f || bad)) {
+          mx *= a.scale_log2;
+          // does any of the 64 threads see a score beyond its row's reference (or know of a wait that ran out)?
+          if (!vote(mx > m_ref + 8.0f || bad)) break;
           s_max[half * 256 + row] = mx;
           if (vote(bad)) {             // both warps leave together: neither may meet the other's barrier alone
-            ok = false;
+            leave = true;
             break;
           }
           mx = fmaxf(mx, s_max[(half ^ 1) * 256 + row]);
@@ -419,7 +418,10 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
           }
           asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");      // s_max may be written again
           tmem_ld32(col_s, xa);                        // the weights again, against the new reference
-          weigh_all();
+        }
+        if (leave) {
+          ok = false;
+          break;
         }
         tmem_st32(col_s, w);
         tmem_wait_st();
