@@ -694,6 +694,8 @@ extern "C" int acache_shared_prefix_attention(const void* q, int64_t q_stride, v
   if (!q || !out || !k_cache || !v_cache || !cu_seqlens_q || !cu_seqlens_k || !scratch || (prefix_len > 0 && !prefix_slots) ||
       (n_slots > 0 && !read_slot_mapping))
     return ACACHE_EINVAL;
+  const float scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (!(scale_log2 > 0.f) || scale_log2 > 3.0e38f) return ACACHE_EINVAL;      // maxima are taken before the scale, dead keys are -inf
   if (dtype == ACACHE_F32 || (head_dim != 64 && head_dim != 128) || q_stride % 8 != 0 || o_stride % 8 != 0 || !aligned16(q) ||
       !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(scratch))
     return ACACHE_EUNSUPPORTED;
@@ -710,7 +712,7 @@ extern "C" int acache_shared_prefix_attention(const void* q, int64_t q_stride, v
   float* o = (float*)scratch;
   float* lse = o + n_parts * n_rows * head_dim;
   const parts::Args a{q, q_stride, k_cache, v_cache, num_slots, n_heads, n_kv_heads, head_dim, dtype,
-                      softmax_scale * 1.4426950408889634f, err_flag, (cudaStream_t)stream};
+                      scale_log2, err_flag, (cudaStream_t)stream};
   const parts::Seg prefix{nullptr, nullptr, prefix_slots, prefix_len, total_q, plan.prefix_splits, prefix_keep, keep_stride, cu_seqlens_q,
                           batch, o, lse, n_rows, 0, plan.prefix_ctas, (int)plan.pre.units, (prefix_len + 127) / 128};
   const parts::Seg own{cu_seqlens_q, cu_seqlens_k, read_slot_mapping, n_slots, total_q, plan.own_splits, nullptr, 0, nullptr, 0, o, lse,

@@ -1,0 +1,43 @@
+"""Host side of shared-prefix attention: no GPU needed."""
+import pytest
+
+
+def _args(**changed):
+    at = 1 << 20                                       # aligned, never dereferenced: every call here is refused or empty
+    args = dict(q=at, q_stride=256, out=at, o_stride=256, k=at, v=at, num_slots=64, total_q=4, n_heads=4, n_kv_heads=2, head_dim=64,
+                dtype=2, prefix_slots=at, prefix_len=10, keep=None, keep_stride=2, cu_q=at, cu_k=at, batch=2, max_q=2, max_k=4,
+                read=at, n_slots=8, scale=0.125, scratch=at, scratch_bytes=0, err=None, stream=None)
+    assert not set(changed) - set(args)
+    return list({**args, **changed}.values())
+
+
+EINVAL, EUNSUPPORTED, ELIMIT = -1, -2, -4
+
+
+@pytest.mark.parametrize("changed,code", [
+    ({}, EINVAL),                                      # no scratch
+    ({"scale": 0.0}, EINVAL), ({"scale": -0.125}, EINVAL), ({"scale": float("nan")}, EINVAL), ({"scale": float("inf")}, EINVAL),
+    ({"scale": 3e38}, EINVAL),                         # infinite in the kernels' base 2
+    ({"n_heads": 3}, EINVAL), ({"q": None}, EINVAL), ({"read": None}, EINVAL), ({"prefix_slots": None}, EINVAL), ({"dtype": 9}, EINVAL),
+    ({"keep": 1 << 20, "keep_stride": 1}, EINVAL), ({"keep": (1 << 20) + 4}, EINVAL), ({"keep": 1 << 20, "prefix_len": 65}, EINVAL),
+    ({"head_dim": 96}, EUNSUPPORTED), ({"dtype": 0}, EUNSUPPORTED), ({"q_stride": 260}, EUNSUPPORTED), ({"q": (1 << 20) + 2}, EUNSUPPORTED),
+    ({"batch": 2048}, ELIMIT), ({"total_q": (1 << 22) + 1}, ELIMIT),
+    ({"total_q": 0}, 0), ({"batch": 0}, 0), ({"max_q": 0}, 0)])
+def test_calls_that_are_refused_or_empty(changed, code):
+    from acache_b200 import _lib
+
+    lib = _lib.load()
+    big = 1 << 60 if changed.get("scale") is not None else 0      # enough scratch: the scale alone is at fault
+    assert lib.acache_shared_prefix_attention(*_args(**{"scratch_bytes": big, **changed})) == code
+
+
+def test_scratch_bytes():
+    from acache_b200 import _lib
+
+    need = _lib.load().acache_shared_prefix_attention_scratch_bytes
+    assert need(0, 4, 2, 64, 1, 1, 1, 1) == 0 and need(4, 3, 2, 64, 1, 1, 1, 1) == 0
+    for sizes in ((1, 1, 1, 64, 1, 1, 0, 0), (1024, 32, 32, 128, 32, 32, 800, 8192), (64, 28, 4, 128, 64, 1, 100, 32768)):
+        total_q, nh, _, D = sizes[:4]
+        row = total_q * nh * (D + 1) * 4
+        assert need(*sizes) % row == 0 and need(*sizes) >= 2 * row
+        assert need(*sizes[:5], 1 << 30, *sizes[6:]) == need(*sizes[:5], total_q, *sizes[6:])   # a request has at most all queries
