@@ -7,9 +7,9 @@
 // memory at the end.  The operands go from global memory straight into the fragments of the m16n8k32 integer
 // products: which k an element belongs to does not matter as long as both operands agree, so the four lanes that
 // share a row each load 16 consecutive bytes of its 64 and feed them to two products as (bytes 0-7) and (bytes 8-15).
-// No staging, no barrier before the end, and one launch (a pair of CTAs on 256-row tcgen05 tiles takes 15 us for 33 x
-// 4096 x 4096 whatever its tile, since one 128-byte k block costs it 0.39 us, and 10 us in 4 K slices with a second launch
-// that adds them; this kernel 8 us, and 4 us for one row: 4.3 TB/s of weights).  gemm_i8.cuh has the rule.
+// No staging, no barrier before the end, and one launch (256-row tcgen05 tiles take 9 us for 33 x 4096 x 4096, since with so few
+// tiles most of their time is the latency of a pair's 32 k blocks; this kernel 7.7 us, and 3.8 us for one row: 4.4 TB/s of
+// weights).  gemm_i8.cuh has the rule.
 #include "gemm_i8.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"

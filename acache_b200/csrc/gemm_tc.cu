@@ -318,6 +318,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   const bool misplaced = (smem_u32(smem_raw) & 1023u) != 0;
+  // Loads and products are issued by an elected lane, for which the compiler makes shorter code than for `lane == 0`: a k block
+  // of 8-bit operands and 128 columns takes 0.25 us instead of 0.39 (16-bit, 512 x 12288 x 4096: 62.3 us instead of 69.6)
+  const bool issues = elect_one();
 
   const int rows_per_tile = 256 * MB;
   const int m_tiles = (p.M + rows_per_tile - 1) / rows_per_tile;
@@ -355,7 +358,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
-    if (lane == 0 && !*abort_flag) {
+    if (issues && !*abort_flag) {
       int s = 0;
       uint32_t round = 0;                      // times the ring has wrapped
       bool ok = true;
@@ -378,7 +381,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ product issuer (leader CTA)
-    if (lane == 0 && rank == 0 && !*abort_flag) {
+    if (issues && rank == 0 && !*abort_flag) {
       uint32_t idesc;
       if constexpr (I8) idesc = make_idesc_i8((uint32_t)BN, 256);
       else idesc = make_idesc(Fmt<T>::id, 0, (uint32_t)BN, 256);
@@ -689,11 +692,13 @@ static int plan_splits(int M, int N, int K) {
   return s < 2 ? 1 : (int)s;
 }
 
-// Tile width and K slices of an 8-bit projection (one 256-row block per pair).  Measured on B200: a 128-byte k block
-// takes a pair 0.39 us whatever its tile's width from 64 to 256 columns (97 ns for each of its four products;
-// 512 x 12288 x 4096: 37-38 us at every width from 128 to 256), so wide tiles do more per k block, and with few of them
-// the K range is sliced: the slices' integer sums cost a second kernel (about 3 us) and their traffic (4 TB/s).  Two row
-// blocks per pair were slower everywhere but at 512 x 4096 x 12288 (29.3 against 29.7 us): their epilogue is exposed.
+// Tile width and K slices of an 8-bit projection (one 256-row block per pair).  Measured on B200: a 128-byte k block takes a
+// pair 0.25 us in a tile of 128 columns, 0.32 at 192 and 0.39 at 256 (0.21 at 64), so wide tiles do more per k block and the
+// narrowest that fills the same whole waves of pairs wins (512 x 4096 x 12288: 24.1 us with 192 columns, 29.3 with 256;
+// 512 x 4096 x 4096: 12.8 with 128, 16.6 with 256).  With few tiles the K range is sliced: the slices' integer sums cost a
+// second kernel, the filling of more pipelines (together about 1 us and 1.2 us per slice) and their traffic (4 TB/s).  Two row
+// blocks per pair were slower everywhere: their epilogue is exposed and they leave room for fewer stages
+// (512 x 4096 x 12288: 27.4 us at best, 4096 x 3584 x 37888: 402 against 353).
 struct Int8Plan { int bn, splits; };
 static Int8Plan plan_int8(int M, int N, int K, int want_bn) {
   const int k_blocks = (K + 127) / 128, m_tiles = (M + 255) / 256;
@@ -706,7 +711,7 @@ static Int8Plan plan_int8(int M, int N, int K, int want_bn) {
       const int per = (k_blocks + s - 1) / s;
       if (s > 1 && (per < 4 || (s - 1) * per >= k_blocks)) continue;       // no empty slice
       const long waves = (tiles * s + kPairs - 1) / kPairs;
-      const double cost = waves * per * (0.36 + bn * 1e-4) + (s > 1 ? 3.0 + s * 2.0e-6 * M * N : 0.0);
+      const double cost = waves * per * std::max(0.21, 0.13 + bn * 1e-3) + (s > 1 ? 1.0 + s * (1.2 + 2.0e-6 * M * N) : 0.0);
       if (cost < best * 0.97) {
         best = cost;
         out = Int8Plan{bn, s};
@@ -893,11 +898,16 @@ extern "C" int acache_linear_int8(const int8_t* x, int64_t x_stride, const float
     return ACACHE_EINVAL;
   gemm::Tile tile{1, plan.bn, 0, 2, 0};
   const int stage_bytes = gemm::A_SUB + plan.bn / 2 * 128;
-  tile.stages = 200 * 1024 / stage_bytes < gemm::kMaxStages ? 200 * 1024 / stage_bytes & ~1 : gemm::kMaxStages;   // handed back in twos
+  // the loads of a stage take 1.7 us from its release to its products, so as many stages as fit; two are handed back per commit,
+  // but wide tiles, whose k blocks take longer than a commit, one by one: that makes 7 stages of them instead of 6
+  // (512 x 12288 x 4096, us: 192 columns 32.2 with 6 stages and 29.0 with 8, 256 columns 30.5 with 6 and 29.4 with 7)
+  const int group = plan.bn > 192 ? 1 : 2;
+  tile.stages = 226 * 1024 / stage_bytes / group * group;
+  if (tile.stages > gemm::kMaxStages) tile.stages = gemm::kMaxStages;
   tile.smem = (size_t)tile.stages * stage_bytes + 512;
   gemm::Params p{};
   p.M = n_rows; p.N = out_features; p.K = in_features; p.MB = 1; p.BN = plan.bn; p.stages = tile.stages;
-  p.acc_stages = 2; p.ksplit = plan.splits; p.group = 2; p.partial = (float*)scratch;
+  p.acc_stages = 2; p.ksplit = plan.splits; p.group = group; p.partial = (float*)scratch;
   CUtensorMap mx, mw;
   if (!tc::make_tensor_map_2d_i8(&mx, x, n_rows, in_features, x_stride, 128) ||
       !tc::make_tensor_map_2d_i8(&mw, weight, out_features, in_features, in_features, plan.bn / 2))
