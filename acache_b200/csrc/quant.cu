@@ -8,17 +8,23 @@
 // never rounded to the model type in between, which the unfused chain does.
 //
 // The quotient t = 127 y / a is formed as y * (127 / a), which is within 2 units of its last place, and
-// its 24 significant bits are rounded to 21.  For 16-bit y and a with significands Y, A < 2^11 the exact
-// t lies on a tie k + 1/2 or at least t / (254 Y) > 2^-19 t from one (the difference is a whole number of
-// units of y's last place over 2a), so rounding to 21 bits restores exact ties and moves nothing else
-// across one: 16-bit rows are quantised as by exact division, at the price of a multiplication.
+// for rows quantised as they are its 24 significant bits are rounded to 21.  For 16-bit y and a with
+// significands Y, A < 2^11 the exact t lies on a tie k + 1/2 or at least t / (254 Y) > 2^-19 t from one
+// (the difference is a whole number of units of y's last place over 2a), so rounding to 21 bits restores
+// exact ties and moves nothing else across one: 16-bit rows are quantised as by exact division, at the
+// price of a multiplication.  Norms and gated values are fp32 results without such ties.
+//
+// A norm's factor rsqrt(mean(x^2) + eps) cancels in q: q = round(127 x w / max|x w|), and only the scale
+// gets it.  So the largest value and the sum of squares are reduced together, behind one barrier.  Where x w or
+// the sum of squares leaves fp32 the row is done again, factor first.
 //
 // A row that holds an infinity or a NaN gets the scale NaN and zeros, so that everything computed
 // from it is NaN; a row of zeros gets the scale 0.
 //
 // A CTA works on a row at a time, one pass over global memory (the row stays in registers), and while it reduces
-// and rounds one row the next one it will take is on its way.  Bound by HBM at size, by latency at the few hundred rows
-// of a decode step: gate 2304 x 12288 28 us (5.0 TB/s), 512 x 12288 8.9 us; norm 4096 x 3584 14.6 us, 512 x 4096 3.3 us.
+// and rounds one row the next one it will take is on its way.  Bound by HBM at size and by a row's chain of reduction,
+// barrier and division at 3-4 thousand columns: gate 2305 x 18944 44 us (5.0 TB/s), 512 x 12288 7.7 us; norm 4096 x 3584
+// 12.5 us (14.6 with two barriers and the factor in every value), 2305 x 3584 7.9 us, 512 x 4096 3.3 us.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -40,26 +46,37 @@ __device__ __forceinline__ float act_fn(float x, int act) {
   return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
 }
 
-// largest |v| as ordered bits: a NaN is larger than an infinity, which is larger than any number
+// max(top, |a|, |b|), a NaN if one of them is
+__device__ __forceinline__ float max_abs(float top, float a, float b) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(top), "f"(a), "f"(b));
+  return m;
+}
+// |v| as bits that order like numbers: a NaN is larger than an infinity, which is larger than any number
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// what a row is shrunk by when its sum of squares leaves fp32: the largest values squared and added stay inside
+constexpr float kShrink = 0x1p-75f;
 
 struct RowScale { float pre, f; bool dead; };   // q = round((v * pre) * f)
 
-__device__ __forceinline__ RowScale row_scale(uint32_t top_bits, float* scale_out) {
+// top_bits: the largest |v| of the row; the row itself is rs * v
+__device__ __forceinline__ RowScale row_scale(uint32_t top_bits, float rs, float* scale_out) {
   RowScale r;
-  const float top = __uint_as_float(top_bits);
-  const bool finite = top_bits < 0x7F800000u;
-  r.pre = top < 0x1p-100f ? 0x1p100f : 1.f;     // keeps 127 / a inside the range of fp32
-  r.dead = !finite || top == 0.f;
+  const float top = __uint_as_float(top_bits), a = top * rs;
+  const bool finite = abs_bits(a) < 0x7F800000u;
+  r.pre = top < 0x1p-100f ? 0x1p100f : 1.f;     // keeps 127 / top inside the range of fp32
+  r.dead = !finite || a == 0.f;
   r.f = r.dead ? 0.f : 127.f / (top * r.pre);
-  if (scale_out) *scale_out = finite ? top / 127.f : __uint_as_float(0x7FC00000u);
+  if (scale_out) *scale_out = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
   return r;
 }
 
-// the quantised value in the low byte (of a row that is not dead)
+// the quantised value of v * pre in the low byte (of a row that is not dead)
+template <bool TIES>
 __device__ __forceinline__ uint32_t quantise(float v, const RowScale& r) {
-  float t = (v * r.pre) * r.f;
-  t = __uint_as_float((__float_as_uint(t) + 4u) & ~7u);     // 21 significant bits
+  float t = v * r.f;
+  if (TIES) t = __uint_as_float((__float_as_uint(t) + 4u) & ~7u);     // 21 significant bits
   return __float_as_uint(t + 0x1.8p23f);
 }
 
@@ -74,6 +91,13 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   return m;
 }
 
+// the warp's sum into its place, to be read behind the next barrier
+__device__ __forceinline__ void warp_sum(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+}
+
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, float* red) {
 #pragma unroll
@@ -86,20 +110,21 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return s;
 }
 
-// CTAs per SM the kernel is compiled and launched for: 1024 threads (1280: norm 2305 x 3584 10.1 us against 9.1; 768: gate
-// 2304 x 12288 32 us against 28), 1536 for rows of one vector a thread
+// CTAs per SM the kernel is compiled and launched for: 1024 threads (1280: norm 2305 x 3584 9.8 us against 8.3; 768: gate
+// 512 x 12288 8.7 us against 7.7), 1536 for rows of one vector a thread
 constexpr int resident(int nt, int vpt) { return vpt == 1 ? 1536 / nt : (vpt <= 4 ? 1024 / nt : 1); }
 
 template <typename T, int SRC, int NT, int VPT>
 __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const Params p) {
   constexpr int E = 16 / sizeof(T);
   constexpr bool TWO = SRC != SRC_ROWS;           // a second input row: up halves, or the residual update
+  constexpr bool TIES = SRC == SRC_ROWS;
   chain_release();
   chain_wait();
   // a thread's vectors of the next row, on their way while it works on the current one (they are its own: no barrier)
-  extern __shared__ __align__(16) uint4 next_row[];      // [TWO ? 2 : 1][VPT][NT]
-  __shared__ float red_sum[NT / 32];
-  __shared__ uint32_t red_max[2][NT / 32];
+  extern __shared__ __align__(16) uint4 next_row[];      // [TWO ? 2 : 1][VPT][NT], and the weights of wide norms, [VPT][NT]
+  __shared__ float red_sum[3][NT / 32];            // two buffers: a fast warp may be one row ahead of a slow one
+  __shared__ uint32_t red_max[3][NT / 32];
   const int tid = threadIdx.x, nvec = p.n_cols / E;
   const bool two = SRC == SRC_GATE || (SRC == SRC_NORM && p.delta);
   auto fetch = [&](int64_t row) {
@@ -115,64 +140,105 @@ __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const P
     }
     tc::cp_async_commit();
   };
+  // the norm's weights, a thread's own vectors again: in registers, but in shared memory where they would spill
+  constexpr bool W_SMEM = VPT > 2;
+  [[maybe_unused]] uint4* weights = next_row + 2 * VPT * NT;
+  [[maybe_unused]] uint4 held[W_SMEM ? 1 : VPT];
   int64_t row = blockIdx.x;
+  if (SRC == SRC_NORM && W_SMEM) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = tid + i * NT;
+      if (c < nvec) tc::cp_async16(tc::smem_u32(weights + c), (const T*)p.weight + (int64_t)c * E, true);
+    }
+  }
   fetch(row);
-  Vec16<T> w[VPT];                                // the norm's weights
-  if (SRC == SRC_NORM) {
+  if (SRC == SRC_NORM && !W_SMEM) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-      if (tid + i * NT < nvec) w[i].u = *reinterpret_cast<const uint4*>((const T*)p.weight + (int64_t)(tid + i * NT) * E);
+      if (tid + i * NT < nvec) held[i] = *reinterpret_cast<const uint4*>((const T*)p.weight + (int64_t)(tid + i * NT) * E);
   }
+  const float inv_cols = 1.f / (float)p.n_cols;
   for (int parity = 0; row < p.n_rows; row += gridDim.x, parity ^= 1) {
     T* xr = (T*)p.x + row * p.x_stride;
-    float y[VPT][E];
-    uint32_t top = 0;
-    float ss = 0.f;
+    float y[VPT][E];                              // SRC_NORM: x * weight, without the row's factor
+    float top = 0.f, ss = 0.f, rs = 1.f;
     tc::cp_async_wait<0>();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = tid + i * NT;
       if (c < nvec) {
-        Vec16<T> a, b;
+        Vec16<T> a, b, w;
         a.u = next_row[i * NT + tid];
+        if (SRC == SRC_NORM) w.u = W_SMEM ? weights[c] : held[W_SMEM ? 0 : i];
         if (TWO && two) b.u = next_row[(VPT + i) * NT + tid];
         if (SRC == SRC_NORM && two) {             // the residual add, rounded to T, written back
 #pragma unroll
           for (int e = 0; e < E; ++e) a.e[e] = from_f32<T>(to_f32<T>(a.e[e]) + to_f32<T>(b.e[e]));
           *reinterpret_cast<uint4*>(xr + (int64_t)c * E) = a.u;
         }
-        if (SRC == SRC_GATE) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) y[i][e] = act_fn(to_f32<T>(a.e[e]), p.act) * to_f32<T>(b.e[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            y[i][e] = to_f32<T>(a.e[e]);
-            if (SRC == SRC_NORM) ss = fmaf(y[i][e], y[i][e], ss);
-          }
+        for (int e = 0; e < E; ++e) {
+          const float v = to_f32<T>(a.e[e]);
+          if (SRC == SRC_NORM) ss = fmaf(v, v, ss);
+          y[i][e] = SRC == SRC_GATE ? act_fn(v, p.act) * to_f32<T>(b.e[e]) : (SRC == SRC_NORM ? v * to_f32<T>(w.e[e]) : v);
         }
-        if (SRC != SRC_NORM) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) top = max(top, abs_bits(y[i][e]));
-        }
+        for (int e = 0; e < E; e += 2) top = max_abs(top, y[i][e], y[i][e + 1]);
       }
     }
     if (row + gridDim.x < p.n_rows) fetch(row + gridDim.x);
+    // one barrier for the row's largest value and, of a norm, its sum of squares
+    if (SRC == SRC_NORM) warp_sum(ss, red_sum[parity]);
+    uint32_t top_bits = block_max<NT>(abs_bits(top), red_max[parity]);
     if (SRC == SRC_NORM) {
-      const float rs = rsqrtf(block_sum<NT>(ss, red_sum) / (float)p.n_cols + p.eps);
+      ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        if (tid + i * NT < nvec) {
+      for (int i = 0; i < NT / 32; ++i) ss += red_sum[parity][i];
+      rs = rsqrtf(ss * inv_cols + p.eps);
+    }
+    RowScale r = row_scale(top_bits, rs, tid == 0 ? p.scale + row : nullptr);
+    if (r.dead || r.pre != 1.f) {                 // rare, and the same for the whole CTA
+      if (SRC == SRC_NORM && (top_bits >= 0x7F800000u || !(ss < INFINITY))) {
+        // x * weight, or the sum of squares, may leave the range of fp32 where the norm does not: the factor first, from the
+        // row in global memory, and the squares of smaller values
+        float k = 1.f;
+        if (!(ss < INFINITY)) {
+          k = kShrink;
+          ss = 0.f;
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            y[i][e] = y[i][e] * rs * to_f32<T>(w[i].e[e]);
-            top = max(top, abs_bits(y[i][e]));
+          for (int i = 0; i < VPT; ++i) {
+            if (tid + i * NT < nvec) {
+              Vec16<T> a;
+              a.u = *reinterpret_cast<const uint4*>(xr + (int64_t)(tid + i * NT) * E);
+#pragma unroll
+              for (int e = 0; e < E; ++e) ss = fmaf(to_f32<T>(a.e[e]) * k, to_f32<T>(a.e[e]) * k, ss);
+            }
+          }
+          rs = rsqrtf(block_sum<NT>(ss, red_sum[2]) * inv_cols + p.eps * k * k);
+        }
+        top = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          if (tid + i * NT < nvec) {
+            Vec16<T> a, w;
+            a.u = *reinterpret_cast<const uint4*>(xr + (int64_t)(tid + i * NT) * E);
+            w.u = W_SMEM ? weights[tid + i * NT] : held[W_SMEM ? 0 : i];
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[i][e] = to_f32<T>(a.e[e]) * k * rs * to_f32<T>(w.e[e]);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) top = max_abs(top, y[i][e], y[i][e + 1]);
           }
         }
+        top_bits = block_max<NT>(abs_bits(top), red_max[2]);
+        r = row_scale(top_bits, 1.f, tid == 0 ? p.scale + row : nullptr);
+        __syncthreads();                          // the third buffers may be written again
       }
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[i][e] *= r.pre;
     }
-    top = block_max<NT>(top, red_max[parity]);    // two buffers: a fast warp may be one row ahead of a slow one
-    const RowScale r = row_scale(top, tid == 0 ? p.scale + row : nullptr);
     int8_t* qr = p.q + row * p.n_cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -182,8 +248,8 @@ __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const P
 #pragma unroll
         for (int g = 0; g < E / 4; ++g) {
           const float* v = &y[i][4 * g];
-          word[g] = __byte_perm(__byte_perm(quantise(v[0], r), quantise(v[1], r), 0x0040),
-                                __byte_perm(quantise(v[2], r), quantise(v[3], r), 0x0040), 0x5410);
+          word[g] = __byte_perm(__byte_perm(quantise<TIES>(v[0], r), quantise<TIES>(v[1], r), 0x0040),
+                                __byte_perm(quantise<TIES>(v[2], r), quantise<TIES>(v[3], r), 0x0040), 0x5410);
           if (r.dead) word[g] = 0;
         }
         if (E == 8) *reinterpret_cast<uint2*>(qr + (int64_t)c * E) = make_uint2(word[0], word[E / 4 - 1]);
@@ -202,7 +268,7 @@ __global__ void __launch_bounds__(256) quantise_any_kernel(const Params p) {
   __shared__ uint32_t red_max[8];
   const int64_t row = blockIdx.x;
   T* xr = (T*)p.x + row * p.x_stride;
-  float ss = 0.f, rs = 0.f;
+  float ss = 0.f, rs = 0.f, k = 1.f;
   if (SRC == SRC_NORM) {
     for (int c = threadIdx.x; c < p.n_cols; c += 256) {
       float v = to_f32<T>(xr[c]);
@@ -213,25 +279,33 @@ __global__ void __launch_bounds__(256) quantise_any_kernel(const Params p) {
       }
       ss = fmaf(v, v, ss);
     }
-    rs = rsqrtf(block_sum<256>(ss, red_sum) / (float)p.n_cols + p.eps);
+    ss = block_sum<256>(ss, red_sum);
+    if (!(ss < INFINITY)) {                           // the squares of smaller values
+      k = kShrink;
+      ss = 0.f;
+      for (int c = threadIdx.x; c < p.n_cols; c += 256) ss = fmaf(to_f32<T>(xr[c]) * k, to_f32<T>(xr[c]) * k, ss);
+      __syncthreads();
+      ss = block_sum<256>(ss, red_sum);
+    }
+    rs = rsqrtf(ss / (float)p.n_cols + p.eps * k * k);
   }
   auto value = [&](int c) {
     const float v = to_f32<T>(xr[c]);
-    if (SRC == SRC_NORM) return v * rs * to_f32<T>(((const T*)p.weight)[c]);
+    if (SRC == SRC_NORM) return v * k * rs * to_f32<T>(((const T*)p.weight)[c]);
     if (SRC == SRC_GATE) return act_fn(v, p.act) * to_f32<T>(xr[p.n_cols + c]);
     return v;
   };
   uint32_t top = 0;
   for (int c = threadIdx.x; c < p.n_cols; c += 256) top = max(top, abs_bits(value(c)));
   top = block_max<256>(top, red_max);
-  const RowScale r = row_scale(top, threadIdx.x == 0 ? p.scale + row : nullptr);
+  const RowScale r = row_scale(top, 1.f, threadIdx.x == 0 ? p.scale + row : nullptr);
   int8_t* qr = p.q + row * p.n_cols;
-  for (int c = threadIdx.x; c < p.n_cols; c += 256) qr[c] = r.dead ? (int8_t)0 : (int8_t)(quantise(value(c), r) & 0xFFu);
+  for (int c = threadIdx.x; c < p.n_cols; c += 256) qr[c] = r.dead ? (int8_t)0 : (int8_t)(quantise<SRC == SRC_ROWS>(value(c) * r.pre, r) & 0xFFu);
 }
 
 template <typename T, int SRC, int NT, int VPT>
 static int launch_row(const Params& p, cudaStream_t st) {
-  constexpr size_t smem = (size_t)(SRC == SRC_ROWS ? 1 : 2) * VPT * NT * 16;
+  constexpr size_t smem = (size_t)(SRC == SRC_ROWS ? 1 : (SRC == SRC_NORM && VPT > 2 ? 3 : 2)) * VPT * NT * 16;
   auto kern = quantise_kernel<T, SRC, NT, VPT>;
   static std::atomic<uint64_t> allowed{0};
   ACACHE_CUDA_CHECK(allow_smem((const void*)kern, smem, allowed));

@@ -416,7 +416,8 @@ def rope_append(q, k, v, positions, inv_freq, k_cache=None, v_cache=None, slot_m
                 attention_factor: float = 1.0):
     """Rotates ``q [n, nh, D]`` and ``k [n, Hkv, D]`` by ``positions`` int64 ``[n]`` times ``inv_freq`` float64
     ``[rotary_dim / 2]`` (on the device, from ``rope_frequencies``) on the first ``rotary_dim`` dimensions of a head,
-    and appends the rotated ``k`` and ``v`` to the paged caches at ``slot_mapping`` int32 ``[n]`` (-1 skips a row).
+    and appends the rotated ``k`` and ``v`` to the paged caches at ``slot_mapping`` int32 ``[n]`` (-1 skips a row; no slot
+    twice).
     Returns the rotated queries (a new tensor; ``q`` and ``k`` stay as they are).  Without caches returns the rotated
     ``(q, k)``.  ``interleaved``: pairs (2j, 2j + 1) instead of (j, j + rotary_dim / 2).  ``attention_factor``
     multiplies sine and cosine.  The table form of the half layout over the whole head is ``rope_store``."""

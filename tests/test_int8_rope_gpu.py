@@ -317,3 +317,29 @@ def test_linear_int8_at_the_edges_of_its_forms(n, k, out):
     ref = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
     assert ((y.double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -21)).all()
     _lib.check_device_errors()
+
+
+@pytest.mark.parametrize("cols", [64, 2048, 3584, 12288, 40000, 50])
+def test_norm_whose_weighted_values_leave_the_range(cols):
+    """x * weight beyond fp32 where the norm is not: the factor has to come first."""
+    from acache_b200 import ops
+
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(5, cols, generator=g) * 2.0 ** 60
+    x[1] *= 2.0 ** -60
+    x[2, 0] = float("nan")
+    x[3] = 0
+    w = torch.randn(cols, generator=g) * 2.0 ** 90
+    x, w = x.to(torch.bfloat16), w.to(torch.bfloat16)
+    q, scale = ops.rmsnorm_int8(x.to(DEV), w.to(DEV), 1e-6)
+    q, scale = q.cpu(), scale.cpu().double()
+    assert torch.isnan(scale[2]) and (q[2:4] == 0).all() and scale[3] == 0
+    rows = [0, 1, 4]
+    y = x.double()[rows]
+    y = y / (y.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+    top = y.abs().amax(1)
+    # scale: the square root of a sum of `cols` squares, a few roundings of 2^-24 each, the sum's in a tree of at most
+    # 128 in line; q: half a step and the same relative error of at most 127 steps
+    rel = 2.0 ** -24 * (128 / 2 + 8)
+    assert ((scale[rows] - top / 127).abs() <= top / 127 * rel).all()
+    assert ((q[rows].double() - 127 * y / top[:, None]).abs() <= 0.5 + 127 * 2 * rel).all()
