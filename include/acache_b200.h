@@ -211,8 +211,9 @@ ACACHE_API int64_t acache_linear_int8_scratch_bytes(int n_rows, int in_features,
  * by attention_factor; the other dimensions are copied.  Angles are formed and reduced in 64 bits, the
  * rotation is in fp32, rounded once.  Rotated queries go to out_q (rows out_q_stride apart).  With
  * slot_mapping, rotated keys and values go to the caches out_k / out_v at slot_mapping[i] (-1 skips the row's
- * k and v; the others are distinct, or a slot ends up with a mix of its rows; any other slot outside [0, num_slots) is skipped and raises err_flag code 1); without it, to row i
- * of the dense out_k[n, n_kv_heads, head_dim] (and out_v, if v is not NULL).  Outputs may not overlap inputs. */
+ * k and v; the others are distinct, or a slot ends up with a mix of its rows; one outside [0, num_slots) is
+ * skipped and raises err_flag code 1); without it, to row i of the dense out_k[n, n_kv_heads, head_dim] (and
+ * out_v, if v is not NULL).  Outputs may not overlap inputs. */
 ACACHE_API int acache_rope_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                                   int64_t v_stride, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int dtype,
                                   const int64_t* positions, const double* inv_freq, int rotary_dim, int interleaved,
