@@ -1,8 +1,8 @@
 // Parts of shared-prefix attention (attention_shared.cu) whose rows fill the tensor cores' tiles: tcgen05 + TMEM,
 // bf16 / fp16, head_dim 64 / 128.
 //
-// A CTA works on (KV head, request and key range, 256 virtual rows), one of them or a share of several; a virtual row is a (query, head-of-the-GQA-group)
-// pair.  The rows are two blocks of 128 that share every staged tile of 128 keys and take turns: while the tensor cores
+// A CTA works on (KV head, request and key range, 256 virtual rows), one of them or a share of several; a virtual row is a
+// (query, head-of-the-GQA-group) pair.  The rows are two blocks of 128 that share every staged tile of 128 keys and take turns: while the tensor cores
 // work on one block's products, the other block's threads are in their softmax.  Roles hand over through mbarriers:
 //   warps 0-15   softmax: two threads per row, one for each half of a tile's keys;
 //   warp 16      issues the products: for one row block after the other O += P(i) V(i), then S(i+1) = Q K(i+1)^T; the warp
@@ -30,8 +30,7 @@
 // products take 64 cycles at N = 128 and 48 at N = 64: 2048 cycles); what a tile costs besides is a fixed chain of TMEM
 // loads, maxima, votes and barriers (a block's softmax about 2600 cycles, 1300 of them exponentials, its products 1100,
 // the hand-overs 700), which is why a tile has 128 keys: with 64 (and two S buffers) 128 keys took 4800 cycles, with one
-// thread per row as with two.  Measured: 7168 rows x 8192 keys, 4 heads (120 GFLOP) in 150 us on the 112 SMs that its 112 CTAs
-// occupy, 0.8 PFLOP/s.
+// thread per row as with two.  Measured: 7168 rows x 8192 keys, 4 heads (120 GFLOP) in 144 us on all 148 SMs, 0.83 PFLOP/s.
 #include "attention_parts.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"

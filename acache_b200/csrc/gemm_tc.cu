@@ -599,7 +599,8 @@ struct Tile { int mb, bn, stages, acc_stages; size_t smem; };
 // on B200 (bf16, operands streaming from L2): a k block is bound by the operand bytes a CTA pulls
 // from L2 -- about 68 GB/s per SM with one row block per CTA (32 KB stages, 6 of them), 57 GB/s with
 // two (48 KB stages, 4 of them) -- and not faster than 0.47 us (one row block) / 0.6 us (two) whatever
-// the tile's width (product issue, commits, the tensor pipe at about 94 ns per 256-row product).
+// the tile's width (product issue, commits, the tensor pipe at about 94 ns per 256-row product).  That was measured before
+// an elected lane issued loads and products, which took 5-10 % off launches of few waves; the choice was not fitted again.
 // A tile whose epilogue cannot overlap the next tile's products (one accumulator stage) pays for it
 // by `exposed` (1.03 for a plain store ... 1.25 for the QKV epilogue).
 static Tile pick_tile(int M, int N, int want_mb, int want_bn, int bn_multiple, double exposed) {

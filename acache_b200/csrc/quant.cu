@@ -1,5 +1,5 @@
 // Rows quantised to 8-bit integers by the kernel that produces them (input side of the 8-bit
-// projections in gemm_i8.cu):
+// projections in gemm_tc.cu and gemm_i8_few.cu):
 //
 //   a_i = max_k |y_ik|      q_ik = round(127 y_ik / a_i), ties to even      scale_i = a_i / 127
 //
