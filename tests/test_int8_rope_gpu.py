@@ -343,3 +343,24 @@ def test_norm_whose_weighted_values_leave_the_range(cols):
     rel = 2.0 ** -24 * (128 / 2 + 8)
     assert ((scale[rows] - top / 127).abs() <= top / 127 * rel).all()
     assert ((q[rows].double() - 127 * y / top[:, None]).abs() <= 0.5 + 127 * 2 * rel).all()
+
+
+@pytest.mark.parametrize("bn", [64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("n,k,out", [(600, 1168, 9472), (300, 4240, 1232), (2000, 128, 9472)])
+def test_linear_int8_rings_that_wrap_inside_tiles(n, k, out, bn):
+    """Several tiles a pair, k blocks that are no multiple of the ring's stages, slices of the K range: every width of the
+    tiles; exact integer sums, two roundings of 2^-24 and one to the output type."""
+    _lib, ops = _ops()
+    g = torch.Generator().manual_seed(n + k)
+    x = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8).to(DEV)
+    w = torch.randint(-128, 128, (out, k), generator=g, dtype=torch.int8).to(DEV)
+    xs, ws = torch.rand(n, generator=g).to(DEV), torch.rand(out, generator=g).to(DEV)
+    ops.GEMM_TILE = (0, bn)
+    try:
+        y = [ops.linear_int8(x, xs, w, ws) for _ in range(3)]
+    finally:
+        ops.GEMM_TILE = (0, 0)
+    ref = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
+    assert ((y[0].double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -21)).all()
+    assert torch.equal(y[0], y[1]) and torch.equal(y[0], y[2])
+    _lib.check_device_errors()
