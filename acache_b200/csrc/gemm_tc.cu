@@ -636,7 +636,8 @@ static Tile pick_tile(int M, int N, int want_mb, int want_bn, int bn_multiple, d
 template <typename T, typename TR, typename TC, int EPI, int MB>
 static int launch_mb(const CUtensorMap& mx, const CUtensorMap& mw, const Params& p, const Tile& tile, cudaStream_t st) {
   auto kern = linear_tc_kernel<T, TR, TC, EPI, MB>;
-  ACACHE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tile.smem));
+  static std::atomic<uint64_t> allowed{0};
+  ACACHE_CUDA_CHECK(allow_smem((const void*)kern, 227 * 1024, allowed));      // whatever the tile needs
   const int m_tiles = (p.M + 256 * p.MB - 1) / (256 * p.MB), n_tiles = (p.N + p.BN - 1) / p.BN;
   const long total = (long)m_tiles * n_tiles * p.ksplit;
   const int pairs = total < kPairs ? (int)total : kPairs;
