@@ -23,7 +23,7 @@
 //
 // A CTA works on a row at a time, one pass over global memory (the row stays in registers), and while it reduces
 // and rounds one row the next one it will take is on its way.  Bound by HBM at size and by a row's chain of reduction,
-// barrier and division at 3-4 thousand columns: gate 2305 x 18944 44 us (5.0 TB/s), 512 x 12288 7.7 us; norm 4096 x 3584
+// barrier and division at 3-4 thousand columns: gate 2304 x 12288 25 us (5.7 TB/s), 512 x 12288 7.7 us; norm 4096 x 3584
 // 12.5 us (14.6 with two barriers and the factor in every value), 2305 x 3584 7.9 us, 512 x 4096 3.3 us.
 #include "common.cuh"
 #include "tcgen05.cuh"
