@@ -592,6 +592,7 @@ static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_l
   p.pre = segment(1, total_q * g, n_kv_heads);
   p.own = segment(batch, max_q * g, n_kv_heads);
   auto splits = [](int64_t slots, int64_t units, int64_t keys, int64_t least) {
+    if (units <= 0) return 1;
     int64_t s = slots / units;
     if (s > keys / least) s = keys / least;
     return (int)(s > 32 ? 32 : (s < 1 ? 1 : s));
@@ -672,9 +673,9 @@ using namespace acache;
 
 extern "C" int64_t acache_shared_prefix_attention_scratch_bytes(int total_q, int n_heads, int n_kv_heads, int head_dim, int batch,
                                                                 int max_seqlen_q, int max_seqlen_k, int prefix_len) {
-  if (total_q <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || batch <= 0 || max_seqlen_q < 0 ||
+  if (total_q <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || batch <= 0 || max_seqlen_q <= 0 ||
       max_seqlen_k < 0 || prefix_len < 0)
-    return 0;
+    return 0;                          // nothing to compute, or a call that is refused
   const shared_prefix::Plan p = shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads);
   const int64_t parts = p.prefix_splits + p.own_splits;
   return parts * total_q * n_heads * (int64_t)(head_dim + 1) * 4;

@@ -225,6 +225,8 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_slots, cu_seqlens_q, cu_
         max_seqlen_q = _max_len(cu_seqlens_q)
     if max_seqlen_k is None:
         max_seqlen_k = _max_len(cu_seqlens_k)
+    if max_seqlen_q == 0:
+        return out                     # a padded batch: no request has a query
     lib = _lib.load()
     with on_device_of(q):
         # the call's own scratch: two streams, or two captured graphs, never share it

@@ -1,5 +1,9 @@
 """Host side of shared-prefix attention: no GPU needed."""
+from pathlib import Path
+
 import pytest
+
+REPO = Path(__file__).resolve().parents[1]
 
 
 def _args(**changed):
@@ -41,3 +45,13 @@ def test_scratch_bytes():
         row = total_q * nh * (D + 1) * 4
         assert need(*sizes) % row == 0 and need(*sizes) >= 2 * row
         assert need(*sizes[:5], 1 << 30, *sizes[6:]) == need(*sizes[:5], total_q, *sizes[6:])   # a request has at most all queries
+
+
+@pytest.mark.parametrize("sizes", [(4, 4, 2, 64, 2, 0, 4, 10), (4, 4, 2, 64, 2, 0, 0, 0), (300, 28, 4, 128, 8, 0, 1024, 32768)])
+def test_requests_without_queries_need_no_scratch(sizes):
+    """A padded batch: rows of q, but no request has one.  In a process of its own: an integer division by zero ends it."""
+    import subprocess
+    import sys
+
+    code = f"from acache_b200 import _lib; assert _lib.load().acache_shared_prefix_attention_scratch_bytes(*{sizes}) == 0"
+    assert subprocess.run([sys.executable, "-c", code], cwd=REPO).returncode == 0

@@ -325,3 +325,25 @@ def test_bad_offsets_stay_inside_the_arrays():
         bad_k[1] = -5
         got = _run(m, q, kc, vc, pre, cu_q, bad_k, slots, None, max_seqlen_q=max(q_lens), max_seqlen_k=30)
         assert torch.isfinite(got).all() and torch.equal(got[cu_q[2]:], want[cu_q[2]:])
+
+
+@pytest.mark.parametrize("n,batch,prefix", [(4, 2, 10), (300, 8, 2000)])
+def test_a_padded_batch_without_queries(n, batch, prefix):
+    """Rows of q behind requests that have none (offsets all zero): the call returns, and nothing of its output is written."""
+    _lib, m = _fn()
+    q, kc, vc, pre, _, cu_k, slots, keep = _inputs([0] * batch, [5] * batch, prefix, 4, 2, 64, BF, drop=0.3)
+    q, cu_q = torch.randn(n, 4, 64).to(BF), torch.zeros(batch + 1, dtype=torch.int32)
+    for kw in ({}, {"max_seqlen_q": 0}, {"max_seqlen_q": 3}):
+        assert _run(m, q, kc, vc, pre, cu_q, cu_k, slots, keep, **kw).shape == q.shape
+    lib = _lib.load()
+    out = torch.full((n, 4, 64), 7.0, dtype=BF, device=DEV)
+    d = [t.to(DEV) for t in (q, kc, vc, pre, cu_q, cu_k, slots)]
+    for max_q in (0, 3):
+        nbytes = lib.acache_shared_prefix_attention_scratch_bytes(n, 4, 2, 64, batch, max_q, 5, prefix)
+        scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=DEV)
+        assert lib.acache_shared_prefix_attention(
+            d[0].data_ptr(), 256, out.data_ptr(), 256, d[1].data_ptr(), d[2].data_ptr(), kc.numel() // 128, n, 4, 2, 64, 2,
+            d[3].data_ptr(), prefix, None, 0, d[4].data_ptr(), d[5].data_ptr(), batch, max_q, 5, d[6].data_ptr(), slots.numel(), 0.125,
+            scratch.data_ptr(), nbytes, None, torch.cuda.current_stream().cuda_stream) == 0
+        assert (out == 7).all()
+    _lib.check_device_errors()
