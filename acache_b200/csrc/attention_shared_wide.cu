@@ -81,9 +81,8 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
   const int quad = warp & 3, rb = (warp >> 2) & 1, half = warp >> 3;
   const int row = rb * BM + quad * 32 + lane;
 
-  // the call's next kernel may start once every CTA is past this point, so that it reads nothing older kernels write
-  chain_wait();
   chain_release();
+  chain_wait();
 
   auto wait_bar = [&](uint32_t at, uint32_t parity) -> bool {      // bounded; ends too when another role has given up
     const long long t0 = clock64();
