@@ -49,8 +49,8 @@ class Config:
     # (``shared_prefix_attention``, instead of ``group_shared_span``) when every request reads it where it is
     # cached; same result up to the order of the floating-point sums
     share_span_once: bool = False
-    # run the projections of the model blocks in 8-bit integers (weights quantised per output channel at start,
-    # activations per token); changes the numbers a model computes, so it is off by default
+    # run the projections of the model blocks in 8-bit integers (weights quantised per output channel at start, into
+    # copies beside the 16-bit parameters that the cache's automatic size takes into account; activations per token); changes the numbers a model computes, so it is off by default
     int8_projections: bool = False
     # anchor selection: probe the newly admitted requests in ragged batches of at most
     # ``max_num_batched_tokens`` query rows (the reference runs one forward per request) and then

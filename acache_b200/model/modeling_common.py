@@ -141,8 +141,11 @@ class FusedProjections:
 
 class Int8Projections:
     """The projections of one block in 8-bit integers (``ops.linear_int8``): copies of the weights quantised per
-    output channel, made again when the parameters were replaced; the activations are quantised per token by the
-    kernel that produces them (norm, gated activation, or ``ops.quantize_rows`` after attention)."""
+    output channel when the object is made; the activations are quantised per token by the kernel that produces them
+    (norm, gated activation, or ``ops.quantize_rows`` after attention).  A projection whose parameters were replaced or
+    written in place since is quantised again at its next call, into the same buffers, so that captured graphs read the new
+    values too.  A write through ``.data`` leaves no trace on a parameter: call ``refresh()`` (a model's ``quantize_int8()``)
+    after it."""
 
     def __init__(self, **projections):
         self.projections = projections              # name -> the nn.Linear modules whose outputs lie side by side
@@ -152,24 +155,51 @@ class Int8Projections:
                 raise ValueError(f"8-bit projections need a 16-bit model on the GPU, not {w.dtype} on {w.device}")
             if w.shape[1] % 16 or sum(m.weight.shape[0] for m in mods) % 16:
                 raise ValueError(f"{name}: the sizes of an 8-bit projection are multiples of 16")
-        self._made = None
+        self._made, self._stamps = {}, {}
+        self.refresh()
 
-    def _params(self):
-        return [p for mods in self.projections.values() for m in mods for p in (m.weight, m.bias)]
+    def _stamp_of(self, name):
+        return FusedProjections._stamp_of([p for m in self.projections[name] for p in (m.weight, m.bias)])
+
+    def refresh(self):
+        """Quantises every projection's present parameters."""
+        for name in self.projections:
+            self._make(name)
+
+    # buffers that can be written again outside of inference mode, whatever mode the first call ran in
+    @torch.inference_mode(False)
+    @torch.no_grad()
+    def _make(self, name):
+        mods = self.projections[name]
+        w = mods[0].weight
+        rows, cols = sum(m.weight.shape[0] for m in mods), w.shape[1]
+        q, scale, bias = self._made.get(name, (None, None, None))
+        if q is None or q.device != w.device:
+            q = torch.empty(rows, cols, dtype=torch.int8, device=w.device)
+            scale = torch.empty(rows, dtype=torch.float32, device=w.device)
+            bias = torch.empty(rows, dtype=w.dtype, device=w.device) if mods[0].bias is not None else None
+            self._made[name] = (q, scale, bias)
+        at = 0
+        for m in mods:
+            part = slice(at, at + m.weight.shape[0])
+            at = part.stop
+            q_part, scale_part = ops.quantize_rows(m.weight.data)
+            q[part].copy_(q_part)
+            scale[part].copy_(scale_part)
+            if bias is not None:
+                bias[part].copy_(m.bias.data)
+        self._stamps[name] = self._stamp_of(name)
 
     def _weights(self):
-        stamp = FusedProjections._stamp_of(self._params())
-        if self._made is None or self._made[0] != stamp:
-            made = {}
-            for name, mods in self.projections.items():
-                parts = [ops.quantize_rows(m.weight.data) for m in mods]
-                bias = torch.cat([m.bias.data for m in mods]) if mods[0].bias is not None else None
-                made[name] = (torch.cat([q for q, _ in parts]), torch.cat([s for _, s in parts]), bias)
-            self._made = (stamp, made)
-        return self._made[1]
+        for name in self.projections:
+            if self._stamps[name] != self._stamp_of(name):
+                self._make(name)
+        return self._made
 
     def __call__(self, name, quantised, dtype):
-        w, scale, bias = self._weights()[name]
+        if self._stamps[name] != self._stamp_of(name):
+            self._make(name)
+        w, scale, bias = self._made[name]
         return ops.linear_int8(quantised[0], quantised[1], w, scale, bias, out_dtype=dtype)
 
 

@@ -105,7 +105,9 @@ class DreamDecoderLayer(nn.Module):
         self.int8 = None        # the projections in 8-bit integers, after quantize_int8()
 
     def quantize_int8(self):
-        """Runs the layer's projections in 8-bit integers from now on."""
+        """Runs the layer's projections in 8-bit integers from now on; called again, quantises the present weights."""
+        if self.int8 is not None:
+            return self.int8.refresh()
         a, m = self.self_attn, self.mlp
         self.int8 = Int8Projections(qkv=(a.q_proj, a.k_proj, a.v_proj), o=(a.o_proj,), gate_up=(m.gate_proj, m.up_proj),
                                     down=(m.down_proj,))

@@ -70,7 +70,9 @@ class LLaDALlamaBlock(nn.Module):
         self._fused.reset(self._projection_params())
 
     def quantize_int8(self):
-        """Runs the block's projections in 8-bit integers from now on."""
+        """Runs the block's projections in 8-bit integers from now on; called again, quantises the present weights."""
+        if self.int8 is not None:
+            return self.int8.refresh()
         self.int8 = Int8Projections(qkv=(self.q_proj, self.k_proj, self.v_proj), attn_out=(self.attn_out,),
                                     gate_up=(self.ff_proj, self.up_proj), ff_out=(self.ff_out,))
 
@@ -199,7 +201,9 @@ class LLaDAModelLM(nn.Module):
 
     def quantize_int8(self):
         """All blocks' projections in 8-bit integers (scales per token and output channel); the embedding and
-        the output head stay as they are.  The 16-bit parameters are kept beside the 8-bit copies."""
+        the output head stay as they are.  The 16-bit parameters are kept beside the 8-bit copies, which are made here.
+        Parameters that are replaced or written in place later are quantised again on their next use; after writes
+        through ``.data``, which leave no trace, call this again."""
         for block in self.model.transformer["blocks"]:
             block.quantize_int8()
         return self

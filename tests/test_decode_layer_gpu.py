@@ -268,3 +268,48 @@ def test_rope_scaling_of_a_model_reaches_tables_and_scores():
         LLaDALlamaBlock(0, LLaDAConfig(d_model=256, n_heads=2, n_kv_heads=2, mlp_hidden_size=64,
                                        rope_scaling=dict(rope_type="dynamic", factor=2.0, original_max_position_embeddings=4096)),
                         None, device=DEV, dtype=BF)
+
+
+@pytest.mark.parametrize("kind", ["llada", "dream"])
+def test_8_bit_weights_are_made_at_start_and_again_when_asked(kind):
+    """The copies exist when ``quantize_int8`` returns (an engine sizes its cache right after); the first forward makes
+    none.  Weights written through ``.data`` are quantised by the next ``quantize_int8``, weights written in place by
+    the next call, both into the buffers that captured graphs read."""
+    from acache_b200 import ops
+    from oracle.models import random_state_dict
+
+    arch = _arch(kind, d_model=1024, n_heads=8, n_kv_heads=8 if kind == "llada" else 2, ffn=4096)
+    _, model = (_llada if kind == "llada" else _dream)(arch, random_state_dict(arch, seed=5, std=0.05), BF)
+    blocks = model.model.transformer["blocks"] if kind == "llada" else model.model.layers
+    linears = [m for b in blocks for m in b.modules() if isinstance(m, torch.nn.Linear)]
+    copies = sum(m.weight.numel() + 4 * m.weight.shape[0] for m in linears)
+    assert copies > 16 << 20
+    # bytes asked for: the allocator does not split a remainder below 1 MB off a block, which memory_allocated() counts
+    held = lambda: torch.cuda.memory_stats()["requested_bytes.all.current"]
+    base = held()
+    model.quantize_int8()
+    assert copies <= held() - base < 1.02 * copies + (1 << 20)
+
+    # what the first use of a projection allocates: its result and scratch
+    before = held()
+    block = blocks[0]
+    x = torch.randn(5, 1024, device=DEV).to(BF)
+    block.int8("gate_up", ops.quantize_rows(x), BF)
+    assert held() - before < copies / 16
+
+    buffers = {n: t[0].data_ptr() for n, t in block.int8._made.items()}
+    w = (block.ff_out if kind == "llada" else block.mlp.down_proj).weight
+    name = "ff_out" if kind == "llada" else "down"
+    h = ops.quantize_rows(torch.randn(5, 4096, device=DEV).to(BF))
+    was = block.int8(name, h, BF)
+    w.data.mul_(2.0)                                   # no trace on the parameter
+    model.quantize_int8()
+    assert torch.equal(block.int8(name, h, BF), was * 2)
+    with torch.no_grad():
+        w.mul_(0.5)
+    with torch.inference_mode():
+        assert torch.equal(block.int8(name, h, BF), was)
+    w.data.mul_(2.0)
+    model.quantize_int8()                              # outside of inference mode again
+    assert torch.equal(block.int8(name, h, BF), was * 2)
+    assert {n: t[0].data_ptr() for n, t in block.int8._made.items()} == buffers
