@@ -13,10 +13,10 @@ def build_rope_table(length: int, head_dim: int, theta: float, dtype: torch.dtyp
     """``(cos, sin)`` tables ``[length, head_dim]`` in the half-split layout
     ``cat(freqs, freqs)`` (reference: nano-vdllm/model/modeling_llada.py:392-402).
     Built once on the host in fp32 so that every device holds identical bits.  With ``scaling`` (a
-    model's ``rope_scaling``, see ``ops.rope_frequencies``) the angles are formed in 64 bits from the
+    model's ``rope_scaling``, see ``ops.rope_frequencies``; "default" is none) the angles are formed in 64 bits from the
     stretched frequencies; an attention factor is not in the tables (``rope_score_factor``), so that
     they stay pure rotations and cached keys can be relocated by further ones."""
-    if scaling is not None:
+    if stretches(scaling):
         inv_freq, _ = model_rope_frequencies(head_dim, theta, scaling)
         freqs = torch.outer(torch.arange(length, dtype=torch.float64), inv_freq)
         emb = torch.cat((freqs, freqs), dim=-1)
@@ -25,6 +25,12 @@ def build_rope_table(length: int, head_dim: int, theta: float, dtype: torch.dtyp
     freqs = torch.outer(torch.arange(length, dtype=torch.float32), inv_freq)
     emb = torch.cat((freqs, freqs), dim=-1)
     return emb.cos().to(dtype).to(device), emb.sin().to(dtype).to(device)
+
+
+def stretches(scaling: dict | None) -> bool:
+    """Whether a configuration's ``rope_scaling`` asks for other frequencies than the plain ones: configuration objects
+    of the transformers package answer ``{"rope_type": "default", ...}`` where none was given."""
+    return scaling is not None and scaling.get("rope_type", scaling.get("type", "default")) != "default"
 
 
 def model_rope_frequencies(head_dim: int, theta: float, scaling: dict):
@@ -37,7 +43,7 @@ def model_rope_frequencies(head_dim: int, theta: float, scaling: dict):
 
 def rope_score_factor(head_dim: int, theta: float, scaling: dict | None) -> float:
     """What a scaling's attention factor (on sine and cosine of queries and keys alike) does to the scores."""
-    return 1.0 if scaling is None else model_rope_frequencies(head_dim, theta, scaling)[1] ** 2
+    return model_rope_frequencies(head_dim, theta, scaling)[1] ** 2 if stretches(scaling) else 1.0
 
 
 # Which projections of the model blocks run on this package's CTA-pair tcgen05 GEMMs

@@ -60,3 +60,16 @@ def test_rope_frequencies():
             rope_frequencies(128, 10000.0, bad)
     with pytest.raises(ValueError):
         rope_frequencies(63, 10000.0)
+
+
+def test_a_default_rope_type_leaves_a_model_as_it_is():
+    """What configuration objects answer where no scaling was given: tables and scores are those without one."""
+    from acache_b200.model.modeling_common import RopeCache, build_rope_table, rope_score_factor
+
+    want = build_rope_table(5000, 128, 500000.0, torch.float32, "cpu")
+    for scaling in (dict(rope_type="default", rope_theta=500000.0), dict(type="default"), {}):
+        got = build_rope_table(5000, 128, 500000.0, torch.float32, "cpu", scaling)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert rope_score_factor(128, 500000.0, scaling) == 1.0
+        cached = RopeCache(128, 500000.0, torch.float32, scaling).get(5000, "cpu")
+        assert torch.equal(cached[1][:5000], want[1])
