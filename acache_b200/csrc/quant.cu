@@ -23,7 +23,7 @@
 //
 // A CTA works on a row at a time, one pass over global memory (the row stays in registers), and while it reduces
 // and rounds one row the next one it will take is on its way.  Bound by HBM at size and by a row's chain of reduction,
-// barrier and division at 3-4 thousand columns: gate 2304 x 12288 25 us (5.7 TB/s), 512 x 12288 7.7 us; norm 4096 x 3584
+// barrier and division at 3-4 thousand columns: gate 2304 x 12288 27 us (5.2 TB/s), 512 x 12288 7.8 us; norm 4096 x 3584
 // 12.5 us (14.6 with two barriers and the factor in every value), 2305 x 3584 7.9 us, 512 x 4096 3.3 us.
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -38,12 +38,56 @@ struct Params {
   int8_t* q; float* scale; int n_rows, n_cols;
 };
 
-__device__ __forceinline__ float act_fn(float x, int act) {
-  // the fast exponential and division (a few units of 2^-22): the value is rounded to 8 bits next, and the exact
-  // forms made the kernel bound by instructions (512 x 12288: 14 us against 9)
-  if (act == 0) return __fdividef(x, 1.f + __expf(-x));
-  if (act == 1) return x > 0.f ? x : (x == x ? 0.f : x);      // a NaN stays
-  return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+// silu(x) = x / (1 + e^-x) for two x down to -80 (below, e^-x leaves fp32).  e^-x is a power of two whose exponent -x log2(e) is
+// formed with what its rounding loses, since an error of d there is one of 0.7 d of the value: within 2^-20 of its value.  Fast
+// powers and reciprocals, two values to an instruction: expf and exact divisions made the kernel bound by instructions
+// (512 x 12288: 14 us against 8).  An infinity gives a NaN, as its row gets a NaN scale either way.
+constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f;      // log2(e) is the two added
+__device__ __forceinline__ uint64_t silu2(uint64_t x) {
+  using namespace tc;
+  float t0, t1, d0, d1;
+  const uint64_t t = mul_f32x2(x, pack_f32x2(kLog2e, kLog2e));
+  uint64_t rest = fma_f32x2(x, pack_f32x2(-kLog2e, -kLog2e), t);                 // what -t lacks of -x log2(e)
+  rest = fma_f32x2(x, pack_f32x2(-kLog2eRest, -kLog2eRest), rest);
+  unpack_f32x2(t, t0, t1);
+  const uint64_t p = pack_f32x2(ex2(-t0), ex2(-t1));
+  const uint64_t e = fma_f32x2(p, mul_f32x2(rest, pack_f32x2(0.69314718f, 0.69314718f)), p);
+  unpack_f32x2(add_f32x2(e, pack_f32x2(1.f, 1.f)), d0, d1);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d1));
+  return mul_f32x2(x, pack_f32x2(d0, d1));
+}
+__device__ __forceinline__ float relu(float x) { return x > 0.f ? x : (x == x ? 0.f : x); }      // a NaN stays
+// gelu(x) = x (1 + erf(x / sqrt 2)) / 2 down to -3: two steps of erff over a sum that cancels, within 2^-14 of its value
+__device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678f)); }
+
+// gates further below zero than this have forms of their own, which would cost the others a tenth (silu) to a third (gelu) more
+__device__ __forceinline__ float far_below(int act) { return act == 0 ? 80.f : (act == 1 ? INFINITY : 3.f); }
+// silu as x e^x / (1 + e^x): within 2^-20 of its value, and 2^-149 |x| below -87, where e^x is subnormal; gelu as
+// x erfc(-x / sqrt 2) / 2: the rounding of the argument counts x^2 times, within (x^2 + 8) 2^-23 of its value
+__device__ __noinline__ float act_far(float x, int act) {
+  if (act != 0) return 0.5f * x * erfcf(x * -0.70710678f);
+  const float t = x * kLog2e, rest = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -t));
+  float p;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(t));       // with subnormal results
+  const float z = fmaf(p, rest * 0.69314718f, p);
+  return __fdividef(x * z, 1.f + z);
+}
+
+// y = act(gate) * up for N values; the gate furthest below zero into `far`
+template <int N>
+__device__ __forceinline__ void gated(const float (&g)[N], const float (&u)[N], int act, float (&y)[N], float& far) {
+  using namespace tc;
+#pragma unroll
+  for (int e = 0; e < N; e += 2) far = max3(far, -g[e], -g[e + 1]);
+  if (act == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2)
+      unpack_f32x2(mul_f32x2(silu2(pack_f32x2(g[e], g[e + 1])), pack_f32x2(u[e], u[e + 1])), y[e], y[e + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = (act == 1 ? relu(g[e]) : gelu(g[e])) * u[e];
+  }
 }
 
 // max(top, |a|, |b|), a NaN if one of them is
@@ -163,6 +207,7 @@ __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const P
     T* xr = (T*)p.x + row * p.x_stride;
     float y[VPT][E];                              // SRC_NORM: x * weight, without the row's factor
     float top = 0.f, ss = 0.f, rs = 1.f;
+    [[maybe_unused]] float far = 0.f;
     tc::cp_async_wait<0>();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -177,14 +222,49 @@ __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const P
           for (int e = 0; e < E; ++e) a.e[e] = from_f32<T>(to_f32<T>(a.e[e]) + to_f32<T>(b.e[e]));
           *reinterpret_cast<uint4*>(xr + (int64_t)c * E) = a.u;
         }
+        if constexpr (SRC == SRC_GATE) {
+          float gate[E], up[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float v = to_f32<T>(a.e[e]);
-          if (SRC == SRC_NORM) ss = fmaf(v, v, ss);
-          y[i][e] = SRC == SRC_GATE ? act_fn(v, p.act) * to_f32<T>(b.e[e]) : (SRC == SRC_NORM ? v * to_f32<T>(w.e[e]) : v);
+          for (int e = 0; e < E; ++e) {
+            gate[e] = to_f32<T>(a.e[e]);
+            up[e] = to_f32<T>(b.e[e]);
+          }
+          gated<E>(gate, up, p.act, y[i], far);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float v = to_f32<T>(a.e[e]);
+            if (SRC == SRC_NORM) ss = fmaf(v, v, ss);
+            y[i][e] = SRC == SRC_NORM ? v * to_f32<T>(w.e[e]) : v;
+          }
         }
+        if constexpr (SRC != SRC_GATE) {
 #pragma unroll
-        for (int e = 0; e < E; e += 2) top = max_abs(top, y[i][e], y[i][e + 1]);
+          for (int e = 0; e < E; e += 2) top = max_abs(top, y[i][e], y[i][e + 1]);
+        }
+      }
+    }
+    if constexpr (SRC == SRC_GATE) {
+      const float limit = far_below(p.act);
+      if (far > limit) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          if (tid + i * NT < nvec) {
+            Vec16<T> a, b;
+            a.u = next_row[i * NT + tid];
+            b.u = next_row[(VPT + i) * NT + tid];
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (-to_f32<T>(a.e[e]) > limit) y[i][e] = act_far(to_f32<T>(a.e[e]), p.act) * to_f32<T>(b.e[e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if (tid + i * NT < nvec) {
+#pragma unroll
+          for (int e = 0; e < E; e += 2) top = max_abs(top, y[i][e], y[i][e + 1]);
+        }
       }
     }
     if (row + gridDim.x < p.n_rows) fetch(row + gridDim.x);
@@ -292,7 +372,12 @@ __global__ void __launch_bounds__(256) quantise_any_kernel(const Params p) {
   auto value = [&](int c) {
     const float v = to_f32<T>(xr[c]);
     if (SRC == SRC_NORM) return v * k * rs * to_f32<T>(((const T*)p.weight)[c]);
-    if (SRC == SRC_GATE) return act_fn(v, p.act) * to_f32<T>(xr[p.n_cols + c]);
+    if (SRC == SRC_GATE) {
+      const float u[2] = {to_f32<T>(xr[p.n_cols + c]), 0.f}, g[2] = {v, 0.f};
+      float y[2], far = 0.f;
+      gated<2>(g, u, p.act, y, far);
+      return far > far_below(p.act) ? act_far(v, p.act) * u[0] : y[0];
+    }
     return v;
   };
   uint32_t top = 0;

@@ -364,3 +364,35 @@ def test_linear_int8_rings_that_wrap_inside_tiles(n, k, out, bn):
     assert ((y[0].double() - ref).abs() <= ref.abs() * (2.0 ** -8 + 2.0 ** -21)).all()
     assert torch.equal(y[0], y[1]) and torch.equal(y[0], y[2])
     _lib.check_device_errors()
+
+
+@pytest.mark.parametrize("cols", [64, 2048, 12288, 50, 40000])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_far_below_zero_that_make_a_row_s_largest_value(act, cols):
+    """Large up values behind gates where the activation is tiny.  silu: a power of two (2^-22), a reciprocal or division
+    (2 steps), four products and a sum, and for -88, where e^x is below the normal range, two steps of 2^-149 of its 2^-127:
+    below 2^-19.  gelu: down to -3 two steps of erff (2^-23) over
+    1 + erf (2^-8.5): 2^-14; below, the rounded argument t = x / sqrt 2 (two roundings of 2^-24) changes erfc by 2 t^2 = x^2
+    times that, erfcf is off by 4 steps, three products."""
+    _lib, ops = _ops()
+    gates = [-20.0, -33.5, -50.0, -64.0, -80.0, -87.0, -88.0] if act == "silu" else [-3.0, -4.0, -5.0, -6.5, -8.0]
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(len(gates), 2 * cols, generator=g)
+    for i, v in enumerate(gates):
+        at = torch.randperm(cols, generator=g)[: cols // 2]
+        x[i, at] = v * (1 - torch.rand(len(at), generator=g) * 2.0 ** -6)
+        x[i, at[0]] = v
+        tiny = float(_act64(torch.tensor([v], dtype=torch.float64), act).abs())
+        x[i, cols + at] = (torch.randn(len(at), generator=g) * 100 / tiny).clamp(-3e38, 3e38)
+    x = x.to(BF)
+    q, s = ops.act_mul_halves_int8(x.to(DEV), act)
+    y = _act64(x[:, :cols].double(), act) if act == "silu" else _gelu64(x[:, :cols].double())
+    y = y * x[:, cols:].double()
+    assert (y.abs().amax(1) > 20).all()                # the gates above decide the scale
+    for i, v in enumerate(gates):
+        rel = 2.0 ** -19 if act == "silu" else (2.0 ** -14 if v >= -3 else (v * v + 8) * 2.0 ** -23)
+        _check_quantised(q[i:i + 1], s[i:i + 1], y[i:i + 1], rel)
+
+
+def _gelu64(x):
+    return 0.5 * x * torch.special.erfc(-x / math.sqrt(2))      # 1 + erf(x / sqrt 2) without its cancellation
