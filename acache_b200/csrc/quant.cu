@@ -12,7 +12,9 @@
 // significands Y, A < 2^11 the exact t lies on a tie k + 1/2 or at least t / (254 Y) > 2^-19 t from one
 // (the difference is a whole number of units of y's last place over 2a), so rounding to 21 bits restores
 // exact ties and moves nothing else across one: 16-bit rows are quantised as by exact division, at the
-// price of a multiplication.  Norms and gated values are fp32 results without such ties.
+// price of a multiplication.  For fp32 rows such a rounding would move values that are no ties (2^-14 of them), so a quotient
+// within its error of a tie is decided in 64 bits, where 127 y and (k + 1/2) a are exact.  Norms and gated values are fp32
+// results without such ties.
 //
 // A norm's factor rsqrt(mean(x^2) + eps) cancels in q: q = round(127 x w / max|x w|), and only the scale
 // gets it.  So the largest value and the sum of squares are reduced together, behind one barrier.  Where x w or
@@ -102,7 +104,7 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // what a row is shrunk by when its sum of squares leaves fp32: the largest values squared and added stay inside
 constexpr float kShrink = 0x1p-75f;
 
-struct RowScale { float pre, f; bool dead; };   // q = round((v * pre) * f)
+struct RowScale { float pre, f, top; bool dead; };   // q = round((v * pre) * f), top the largest |v * pre|
 
 // top_bits: the largest |v| of the row; the row itself is rs * v
 __device__ __forceinline__ RowScale row_scale(uint32_t top_bits, float rs, float* scale_out) {
@@ -111,17 +113,31 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits, float rs, float
   const bool finite = abs_bits(a) < 0x7F800000u;
   r.pre = top < 0x1p-100f ? 0x1p100f : 1.f;     // keeps 127 / top inside the range of fp32
   r.dead = !finite || a == 0.f;
-  r.f = r.dead ? 0.f : 127.f / (top * r.pre);
+  r.top = top * r.pre;
+  r.f = r.dead ? 0.f : 127.f / r.top;
   if (scale_out) *scale_out = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
   return r;
 }
 
-// the quantised value of v * pre in the low byte (of a row that is not dead)
-template <bool TIES>
+// round(127 v / top) of a quotient t that lies near a tie
+__device__ __noinline__ uint32_t round_near_tie(float v, float t, float top) {
+  const int k = (int)floorf(fabsf(t) - 0.25f);          // between k and k + 1
+  const double x = 127.0 * fabsf(v), tie = (k + 0.5) * top;
+  const int q = k + (x > tie || (x == tie && (k & 1)));
+  return (uint32_t)(v < 0.f ? -q : q);
+}
+
+// the quantised value of v * pre in the low byte (of a row that is not dead).  How a quotient next to a tie is rounded:
+enum { AS_IT_IS = 0, TIES_16 = 1, TIES_32 = 2 };        // T a 16-bit type: 21 significant bits; fp32: exactly
+template <typename T, int SRC> constexpr int kTies = SRC != SRC_ROWS ? AS_IT_IS : (sizeof(T) == 2 ? TIES_16 : TIES_32);
+template <int TIES>
 __device__ __forceinline__ uint32_t quantise(float v, const RowScale& r) {
   float t = v * r.f;
-  if (TIES) t = __uint_as_float((__float_as_uint(t) + 4u) & ~7u);     // 21 significant bits
-  return __float_as_uint(t + 0x1.8p23f);
+  if (TIES == TIES_16) t = __uint_as_float((__float_as_uint(t) + 4u) & ~7u);
+  const float shifted = t + 0x1.8p23f;
+  // t is within 2^-16 of the quotient
+  if (TIES == TIES_32 && fabsf(t - (shifted - 0x1.8p23f)) > 0.5f - 0x1p-15f) return round_near_tie(v, t, r.top);
+  return __float_as_uint(shifted);
 }
 
 template <int NT>
@@ -162,7 +178,7 @@ template <typename T, int SRC, int NT, int VPT>
 __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const Params p) {
   constexpr int E = 16 / sizeof(T);
   constexpr bool TWO = SRC != SRC_ROWS;           // a second input row: up halves, or the residual update
-  constexpr bool TIES = SRC == SRC_ROWS;
+  constexpr int TIES = kTies<T, SRC>;
   chain_release();
   chain_wait();
   // a thread's vectors of the next row, on their way while it works on the current one (they are its own: no barrier)
@@ -385,7 +401,7 @@ __global__ void __launch_bounds__(256) quantise_any_kernel(const Params p) {
   top = block_max<256>(top, red_max);
   const RowScale r = row_scale(top, 1.f, threadIdx.x == 0 ? p.scale + row : nullptr);
   int8_t* qr = p.q + row * p.n_cols;
-  for (int c = threadIdx.x; c < p.n_cols; c += 256) qr[c] = r.dead ? (int8_t)0 : (int8_t)(quantise<SRC == SRC_ROWS>(value(c) * r.pre, r) & 0xFFu);
+  for (int c = threadIdx.x; c < p.n_cols; c += 256) qr[c] = r.dead ? (int8_t)0 : (int8_t)(quantise<kTies<T, SRC>>(value(c) * r.pre, r) & 0xFFu);
 }
 
 template <typename T, int SRC, int NT, int VPT>

@@ -396,3 +396,33 @@ def test_gates_far_below_zero_that_make_a_row_s_largest_value(act, cols):
 
 def _gelu64(x):
     return 0.5 * x * torch.special.erfc(-x / math.sqrt(2))      # 1 + erf(x / sqrt 2) without its cancellation
+
+
+@pytest.mark.parametrize("n,cols", [(3, 4096), (2, 1003), (2, 33000), (40, 256)])
+def test_quantize_rows_is_exact_for_fp32_rows(n, cols):
+    """Values next to ties k + 1/2, one to many steps of fp32 above and below, and exact ties: 127 x and (k + 1/2) a are exact in 64
+    bits (31 and 32 significant bits), so the expected integer is too."""
+    _lib, ops = _ops()
+    g = torch.Generator().manual_seed(cols)
+    top = (1 + torch.rand(n, 1, generator=g)) * torch.exp2(torch.randint(-120, 120, (n, 1), generator=g).float())
+    if n > 9:
+        top[9] *= 2.0 ** -30                           # subnormal for the smallest exponents
+        top[8] = 2.0 ** -140
+    top[0] = 127.0                                     # exact ties exist: x = k + 1/2
+    k = torch.randint(0, 127, (n, cols), generator=g).double()
+    x = ((k + 0.5) * top.double() / 127).float()
+    steps = torch.randint(-3, 4, (n, cols), generator=g)
+    far = torch.rand(n, cols, generator=g) < 0.3
+    steps = torch.where(far, steps * 37, steps)
+    x = (x.view(torch.int32) + steps.to(torch.int32)).clamp_min(0).view(torch.float32)
+    x[0, ::3] = (k[0, ::3] + 0.5).float()
+    x = torch.minimum(x, top) * (1 - 2 * (torch.rand(n, cols, generator=g) < 0.5).float())
+    x[:, cols // 2] = top[:, 0]
+    t = 127 * x.double().abs()
+    m = (t / top.double()).floor()
+    tie = (m + 0.5) * top.double()
+    want = (m + ((t > tie) | ((t == tie) & (m % 2 == 1)))) * x.double().sign()
+    assert (t == tie).any() and ((t / top.double()) % 1 - 0.5).abs().median() < 2.0 ** -13
+    for rows in (x.to(DEV), torch.nn.functional.pad(x.to(DEV), (1, 0))[:, 1:]):       # both kernels
+        q, _ = ops.quantize_rows(rows)
+        assert torch.equal(q.cpu().double(), want)
