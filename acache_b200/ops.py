@@ -356,11 +356,12 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
         lib = _lib.load()
         with on_device_of(x):
             # the sums of K slices, where the launch cuts the K range: a tensor of this call's own
-            nbytes = lib.acache_linear_int8_scratch_bytes(n, k, N, GEMM_TILE[1])
+            bn = GEMM_TILE[1] if GEMM_TILE[1] % 32 == 0 and 64 <= GEMM_TILE[1] <= 256 else 0     # other widths: 16-bit tiles only
+            nbytes = lib.acache_linear_int8_scratch_bytes(n, k, N, bn)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             check(lib.acache_linear_int8(
                 ptr(x), x.stride(0), ptr(x_scale), n, k, ptr(weight), ptr(weight_scale), N, ptr(bias), dtype_code(out_dtype),
-                ptr(out), N, GEMM_TILE[1], ptr(scratch), nbytes, ptr(_lib.err_flag(dev)), stream_ptr()), "linear_int8",
+                ptr(out), N, bn, ptr(scratch), nbytes, ptr(_lib.err_flag(dev)), stream_ptr()), "linear_int8",
                 2 if nbytes else 1)
     return out
 

@@ -426,3 +426,18 @@ def test_quantize_rows_is_exact_for_fp32_rows(n, cols):
     for rows in (x.to(DEV), torch.nn.functional.pad(x.to(DEV), (1, 0))[:, 1:]):       # both kernels
         q, _ = ops.quantize_rows(rows)
         assert torch.equal(q.cpu().double(), want)
+
+
+@pytest.mark.parametrize("tile", [(1, 80), (2, 16), (0, 48)])
+def test_a_tile_width_of_the_16_bit_projections_leaves_linear_int8_alone(tile):
+    """``GEMM_TILE`` serves both families; widths that only the 16-bit kernels have mean the automatic choice here."""
+    _lib, ops = _ops()
+    x = torch.randint(-128, 128, (300, 256), dtype=torch.int8, device=DEV)
+    w = torch.randint(-128, 128, (512, 256), dtype=torch.int8, device=DEV)
+    xs, ws = torch.rand(300, device=DEV), torch.rand(512, device=DEV)
+    want = ops.linear_int8(x, xs, w, ws)
+    ops.GEMM_TILE = tile
+    try:
+        assert torch.equal(ops.linear_int8(x, xs, w, ws), want)
+    finally:
+        ops.GEMM_TILE = (0, 0)
