@@ -1,4 +1,4 @@
-// 8-bit projection for few rows (at most 64: the last running requests of a decode batch), bound by the bytes of
+// 8-bit projection for few rows (at most 48: the last running requests of a decode batch), bound by the bytes of
 // the weight matrix:
 //
 //   out[i, j] = (sum_k x[i, k] w[j, k]) * x_scale[i] * w_scale[j] (+ bias[j]),   sums exact in 32-bit integers
@@ -134,8 +134,7 @@ static int launch(const Params& p, cudaStream_t st) {
   switch ((p.M + 15) / 16) {
     case 1: return launch_mt<T, 1>(p, st);
     case 2: return launch_mt<T, 2>(p, st);
-    case 3: return launch_mt<T, 3>(p, st);
-    default: return launch_mt<T, 4>(p, st);
+    default: return launch_mt<T, 3>(p, st);            // the rule takes at most 48 rows
   }
 }
 

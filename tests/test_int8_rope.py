@@ -73,3 +73,15 @@ def test_a_default_rope_type_leaves_a_model_as_it_is():
         assert rope_score_factor(128, 500000.0, scaling) == 1.0
         cached = RopeCache(128, 500000.0, torch.float32, scaling).get(5000, "cpu")
         assert torch.equal(cached[1][:5000], want[1])
+
+
+def test_few_rows_of_a_narrow_projection_with_a_long_k_range_are_sliced():
+    """One CTA per 32 columns would stream the whole weight matrix through a few SMs: the K range goes to the tiles that cut
+    it into slices, whose sums need scratch."""
+    from acache_b200 import _lib
+
+    need = _lib.load().acache_linear_int8_scratch_bytes
+    for rows, k, out in ((1, 131056, 64), (3, 131056, 32), (16, 32768, 256), (32, 16384, 1024), (64, 12288, 4096)):
+        assert need(rows, k, out, 0) >= 2 * rows * out * 4, (rows, k, out)
+    for rows, k, out in ((1, 4096, 4096), (16, 12288, 4096), (33, 4096, 4096), (32, 18944, 3584)):
+        assert need(rows, k, out, 0) == 0, (rows, k, out)
