@@ -1114,6 +1114,9 @@ class ModelRunner(DkvMixin):
                 keep[i, :span] = attention_read_runs(s)[0][:span] >= 0
             arrays["prefix"] = np.arange(first, first + span, dtype=np.int32)
             arrays["keep"] = np.packbits(keep, axis=1, bitorder="little").view(np.int32)
+            # the longest request's own keys in steps of the attention's shortest key range: its plan follows from this bound,
+            # eagerly and in the graph that is kept for it, so both add in the same order
+            own_bound = -(-int(np.diff(cu_k).max()) // 256) * 256
         elif use_qr or grouped:
             arrays["shared_lens"] = np.asarray(shared_lens, dtype=np.int32)
         if not materialized:
@@ -1121,8 +1124,8 @@ class ModelRunner(DkvMixin):
         staging = self._staging
         self._decode_graph = None
         if graphs is not None:
-            # a shared span's length is part of the captured launches
-            key = (len(ps), grouped, arrays["prefix"].size if once else 0, tuple(sorted(arrays)))
+            # a shared span's length and the bound on the own keys are part of the captured launches
+            key = (len(ps), grouped, (arrays["prefix"].size, own_bound) if once else 0, tuple(sorted(arrays)))
             graph = graphs.get(key)
             if graph is None or not graph.staging.fits(**arrays):
                 # read-map capacity and RoPE table length: powers of two with head-room
@@ -1144,11 +1147,10 @@ class ModelRunner(DkvMixin):
         if once:
             ctx = get_context()
             ctx.shared_prefix = (dev["prefix"], dev["keep"])
-            ctx.max_seqlen_k = int(np.diff(cu_k).max())
+            ctx.max_seqlen_k = own_bound
             if self._decode_graph is not None:
-                # the launches that are captured serve every later step: sizes as the buffers allow, not as this step has them
+                # the launches that are captured serve every later step: the length the buffer allows, not this step's
                 ctx.read_slot_mapping = self._decode_graph.staging.whole("read")
-                ctx.max_seqlen_k = self._decode_graph.max_pos
         return dev["positions"]
 
     # Every captured decode forward keeps its own logits tensor ``[rows * block_length, vocab]`` alive

@@ -313,3 +313,82 @@ def test_8_bit_weights_are_made_at_start_and_again_when_asked(kind):
     model.quantize_int8()                              # outside of inference mode again
     assert torch.equal(block.int8(name, h, BF), was * 2)
     assert {n: t[0].data_ptr() for n, t in block.int8._made.items()} == buffers
+
+
+@pytest.mark.parametrize("kind,A,G", [("llada", 300, 16), ("dream", 700, 24), ("llada", 70, 600)])
+def test_the_shared_span_s_layout_and_plan_in_eager_steps_and_graphs(kind, A, G):
+    """``share_span_once``, every decode step: the kept span keys and the own keys of a request are exactly the slots of its
+    read map; the operator's result is the per-request operator's on those slots (both round weights and result to the
+    type); the bound it plans for is that of the own keys, within 256, eager or captured; replayed tokens equal eager ones."""
+    from acache_b200 import _lib
+    from acache_b200.model import acache_attention as aa
+    from acache_b200.model import attention as at
+    from acache_b200.model_runner import ModelRunner
+    from acache_b200.sequence import Sequence
+    from acache_b200.utils import get_context
+    from oracle.models import random_state_dict
+
+    arch = _arch(kind)
+    weights = random_state_dict(arch, seed=11, std=0.2)
+    T = 8
+    rng = random.Random(A)
+    affix = [rng.randint(1, 170) for _ in range(A)]
+    reqs = _random_requests(rng, arch, 6, A, G, ["prefix"], affix)
+    hf_cfg, model = (_llada if kind == "llada" else _dream)(arch, weights, BF)
+    eps, state, bounds = torch.finfo(BF).eps, {}, {False: set(), True: set()}
+
+    def spied(q, kc, vc, prefix, cu_q, cu_k, read, scale, *, prefix_keep, max_seqlen_q, max_seqlen_k):
+        out = aa.shared_prefix_attention(q, kc, vc, prefix, cu_q, cu_k, read, scale, prefix_keep=prefix_keep,
+                                         max_seqlen_q=max_seqlen_q, max_seqlen_k=max_seqlen_k)
+        bounds[state["graphs"]].add(max_seqlen_k)
+        if not state["graphs"]:
+            longest = max(state["lens"])
+            assert longest <= max_seqlen_k < longest + 256
+            cu = torch.tensor([0, *itertools.accumulate(len(m) for m in state["maps"])], dtype=torch.int32, device=DEV)
+            slots = torch.tensor([x for m in state["maps"] for x in m], dtype=torch.int32, device=DEV)
+            other = aa.acache_attention(q, kc, vc, cu_q, cu, slots, scale).double()
+            size = aa.acache_attention(q, kc, vc.abs(), cu_q, cu, slots, scale).double() * (1 + eps)
+            tol = 2 * (other.abs() * eps / 2 + size * (eps / 2 + 2.0 ** -15)) + other.abs() * eps ** 2
+            assert ((out.double() - other).abs() <= tol).all()
+            state["checked"] = state.get("checked", 0) + 1
+        return out
+
+    def serve(graphs):
+        state["graphs"] = graphs
+        cfg = _serve_config(hf_cfg, arch, kind, BF, threshold=0.6, anchor_ratio=0.2, max_num_seqs=4, num_kvcache_blocks=120,
+                            cache_block_size=64, block_length=T, gen_length=G, share_span_once=True, use_cuda_graphs=graphs)
+        runner = ModelRunner(model, cfg)
+        real = runner.prepare_decoding_acache
+
+        def prepare(seqs, active_indices=None, graphs=None):
+            positions = real(seqs, active_indices, graphs=graphs)
+            ctx, ps = get_context(), runner._pick(seqs, active_indices)
+            if ctx.shared_prefix is not None:
+                prefix, words = (t.cpu() for t in ctx.shared_prefix)
+                bits = (words[:, :, None] >> torch.arange(32)) & 1
+                keep = bits.flatten(1)[:, :prefix.numel()].bool()
+                cu, read = ctx.cu_seqlens_k.tolist(), ctx.read_slot_mapping.cpu()
+                state["maps"] = [[int(x) for x in s.read_slot_map] for s in ps]
+                state["lens"] = [b - a for a, b in zip(cu, cu[1:])]
+                for i, s in enumerate(ps):
+                    assert len(state["maps"][i]) == len(s)
+                    assert sorted(prefix[keep[i]].tolist() + read[cu[i]:cu[i + 1]].tolist()) == sorted(state["maps"][i])
+            return positions
+
+        runner.prepare_decoding_acache = prepare
+        seqs = [Sequence(r["prompt"], block_length=T, gen_length=G, cache_block_size=64, mask_id=arch.mask_id,
+                         prompt_affix_start=r["affix_start"], prompt_affix_end=r["affix_end"],
+                         generation_start=r["generation_start"]) for r in reqs]
+        outs, _ = runner.generate_with_acache(seqs)
+        _lib.check_device_errors()
+        return outs
+
+    old, at.shared_prefix_attention = at.shared_prefix_attention, spied
+    try:
+        eager = serve(False)
+        assert state["checked"] > 0
+        replayed = serve(True)
+    finally:
+        at.shared_prefix_attention = old
+    assert bounds[True] <= bounds[False] and bounds[True]
+    assert replayed == eager
