@@ -392,3 +392,73 @@ def test_the_shared_span_s_layout_and_plan_in_eager_steps_and_graphs(kind, A, G)
         at.shared_prefix_attention = old
     assert bounds[True] <= bounds[False] and bounds[True]
     assert replayed == eager
+
+
+@pytest.mark.parametrize("kind,nh,hkv", [("llada", 4, 4), ("dream", 4, 2)])
+@pytest.mark.parametrize("max_num_seqs", [1, 4])
+@pytest.mark.parametrize("scaling", [dict(rope_type="linear", factor=4.0),
+                                     dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=64)])
+def test_engine_with_rope_scaling_equals_the_oracle(kind, nh, hkv, max_num_seqs, scaling, monkeypatch):
+    """A model with stretched frequencies in fp32, affixes at the start, inside and at the end (cached keys are relocated, by
+    query or into copies): greedy tokens and anchors of the CPU restatement with the same frequencies, whose queries carry
+    the attention factor of queries and keys."""
+    import functools
+
+    import oracle.engine
+    import oracle.models
+    from acache_b200 import _lib, ops
+    from acache_b200.model import configuration
+    from acache_b200.model_runner import ModelRunner
+    from acache_b200.sequence import Sequence
+    from oracle.models import ArchSpec, OracleModel, random_state_dict
+    from oracle.rope import apply_rope
+
+    rng = random.Random(5)
+    arch = ArchSpec(kind, n_layers=2, d_model=64, n_heads=nh, n_kv_heads=hkv, ffn=96, vocab=160, rope_theta=10000.0,
+                    rms_eps=1e-5 if kind == "llada" else 1e-6, act="silu", mask_id=159)
+    inv, factor = ops.rope_frequencies(16, 10000.0, scaling)
+
+    def table(length, head_dim, theta, dtype=torch.float32):
+        assert head_dim == 16 and theta == 10000.0
+        angle = torch.arange(length, dtype=torch.float64)[:, None] * torch.cat([inv, inv])
+        return angle.cos().to(dtype), angle.sin().to(dtype)
+
+    def rope_qk(q, k, positions, theta):
+        cos, sin = table(int(positions.max()) + 1, q.shape[-1], theta)
+        return apply_rope(q, cos[positions], sin[positions]) * factor ** 2, apply_rope(k, cos[positions], sin[positions])
+
+    monkeypatch.setattr(oracle.engine, "rope_table", table)
+    monkeypatch.setattr(oracle.models, "llada_rope_qk", rope_qk)
+    monkeypatch.setattr(oracle.models, "dream_rope_qk", rope_qk)
+    for name in ("LLaDAConfig", "DreamConfig"):
+        monkeypatch.setattr(configuration, name, functools.partial(getattr(configuration, name), rope_scaling=scaling))
+    weights = random_state_dict(arch, seed=11, std=0.3)
+    A, G, T = 13, 8, 4
+    affix = [rng.randint(1, 150) for _ in range(A)]
+    reqs = _random_requests(rng, arch, 6, A, G, ["infix", "prefix", "suffix"], affix)
+
+    def expected():
+        o_req = []
+        for r in reqs:
+            toks = list(r["prompt"]) + ([arch.mask_id] * G if r["generation_start"] is None else [])
+            o_req.append(dict(tokens=toks, affix_start=r["affix_start"], affix_end=r["affix_end"],
+                              generation_start=len(r["prompt"]) if r["generation_start"] is None else r["generation_start"],
+                              gen_length=G))
+        return oracle.engine.generate_with_acache(OracleModel(arch, weights, torch.float32), o_req, anchor_ratio=0.3,
+                                                  threshold=0.6, block_length=T)
+
+    want, want_nfe, want_anchors = expected()
+    hf_cfg, model = (_llada if kind == "llada" else _dream)(arch, weights, torch.float32)
+    cfg = _serve_config(hf_cfg, arch, kind, torch.float32, threshold=0.6, anchor_ratio=0.3, max_num_seqs=max_num_seqs,
+                        num_kvcache_blocks=32, block_length=T, gen_length=G)
+    runner = ModelRunner(model, cfg)
+    seqs = [Sequence(r["prompt"], block_length=T, gen_length=G, cache_block_size=8, mask_id=arch.mask_id,
+                     prompt_affix_start=r["affix_start"], prompt_affix_end=r["affix_end"],
+                     generation_start=r["generation_start"]) for r in reqs]
+    outs, nfe = runner.generate_with_acache(seqs)
+    _lib.check_device_errors()
+    assert [s.anchor_positions for s in seqs] == want_anchors
+    assert outs == want and nfe == want_nfe
+    # the frequencies matter: the plain ones give other tokens
+    monkeypatch.undo()
+    assert expected()[0] != want

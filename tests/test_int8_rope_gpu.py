@@ -441,3 +441,11 @@ def test_a_tile_width_of_the_16_bit_projections_leaves_linear_int8_alone(tile):
         assert torch.equal(ops.linear_int8(x, xs, w, ws), want)
     finally:
         ops.GEMM_TILE = (0, 0)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("n,nh,hkv,D,rot", [(1, 2, 1, 128, 128), (33, 4, 2, 64, 32), (6, 3, 1, 40, 24), (4, 2, 2, 128, 0), (7, 1, 1, 12, 8),
+                                           (5, 2, 1, 256, 64)])
+def test_rope_append_vectors_of_fp32(n, nh, hkv, D, rot, interleaved):
+    """Rows that whole 16-byte vectors of four values fit, on which the vector kernel runs (heads beyond 128: the other one)."""
+    test_rope_append(n, nh, hkv, D, rot, torch.float32, interleaved)
