@@ -80,6 +80,7 @@ _SIGNATURES = {
                                          c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                          c_int, c_void_p, c_int64, c_void_p, c_void_p]),
     "acache_shared_prefix_attention_scratch_bytes": (c_int64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "acache_shared_prefix_attention_plan": (c_int64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "acache_shared_prefix_attention": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int,
                                                c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_void_p,
                                                c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_float, c_void_p,

@@ -667,14 +667,21 @@ static int run(const parts::Args& a, const parts::Seg& prefix, const parts::Seg&
 
 using namespace acache;
 
-extern "C" int64_t acache_shared_prefix_attention_scratch_bytes(int total_q, int n_heads, int n_kv_heads, int head_dim, int batch,
-                                                                int max_seqlen_q, int max_seqlen_k, int prefix_len) {
+extern "C" int64_t acache_shared_prefix_attention_plan(int total_q, int n_heads, int n_kv_heads, int head_dim, int batch,
+                                                       int max_seqlen_q, int max_seqlen_k, int prefix_len, int32_t* launches) {
+  if (launches) *launches = 0;
   if (total_q <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || batch <= 0 || max_seqlen_q <= 0 ||
       max_seqlen_k < 0 || prefix_len < 0)
     return 0;                          // nothing to compute, or a call that is refused
   const shared_prefix::Plan p = shared_prefix::make_plan(total_q, batch, max_seqlen_q, max_seqlen_k, prefix_len, n_heads, n_kv_heads);
   const int64_t parts = p.prefix_splits + p.own_splits;
+  if (launches) *launches = (prefix_len > 0) + 1 + !p.final;
   return parts * total_q * n_heads * (int64_t)(head_dim + 1) * 4;
+}
+
+extern "C" int64_t acache_shared_prefix_attention_scratch_bytes(int total_q, int n_heads, int n_kv_heads, int head_dim, int batch,
+                                                                int max_seqlen_q, int max_seqlen_k, int prefix_len) {
+  return acache_shared_prefix_attention_plan(total_q, n_heads, n_kv_heads, head_dim, batch, max_seqlen_q, max_seqlen_k, prefix_len, nullptr);
 }
 
 extern "C" int acache_shared_prefix_attention(const void* q, int64_t q_stride, void* out, int64_t o_stride, const void* k_cache,

@@ -14,6 +14,8 @@ Differences a caller can see:
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from .. import _lib
@@ -230,14 +232,16 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_slots, cu_seqlens_q, cu_
     lib = _lib.load()
     with on_device_of(q):
         # the call's own scratch: two streams, or two captured graphs, never share it
-        nbytes = lib.acache_shared_prefix_attention_scratch_bytes(total_q, nh, hkv, D, batch, max_seqlen_q, max_seqlen_k, P)
+        launches = ctypes.c_int32()
+        nbytes = lib.acache_shared_prefix_attention_plan(total_q, nh, hkv, D, batch, max_seqlen_q, max_seqlen_k, P,
+                                                         ctypes.byref(launches))
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _lib.timed("attention_decode" if ATTENTION_PHASE == "decode" else "attention_refresh", ATTENTION_WORK):
             check(lib.acache_shared_prefix_attention(
                 ptr(q), q_stride, ptr(out), nh * D, ptr(k_cache), ptr(v_cache), k_cache.numel() // (hkv * D), total_q, nh,
                 hkv, D, dtype_code(dtype), ptr(prefix_slots), P, ptr(prefix_keep), keep_stride, ptr(cu_seqlens_q),
                 ptr(cu_seqlens_k), batch, max_seqlen_q, max_seqlen_k, ptr(read_slot_mapping), n_slots, softmax_scale,
-                ptr(scratch), nbytes, ptr(_lib.err_flag(dev)), stream_ptr()), "shared_prefix_attention", 3)
+                ptr(scratch), nbytes, ptr(_lib.err_flag(dev)), stream_ptr()), "shared_prefix_attention", launches.value)
     return out
 
 

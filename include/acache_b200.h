@@ -376,6 +376,10 @@ ACACHE_API int acache_attention_grouped(const void* q, int64_t q_stride, void* o
 ACACHE_API int64_t acache_shared_prefix_attention_scratch_bytes(int total_q, int n_heads, int n_kv_heads, int head_dim,
                                                                 int batch, int max_seqlen_q, int max_seqlen_k,
                                                                 int prefix_len);
+/* the same, and how many kernels the call launches (launches may be NULL) */
+ACACHE_API int64_t acache_shared_prefix_attention_plan(int total_q, int n_heads, int n_kv_heads, int head_dim, int batch,
+                                                       int max_seqlen_q, int max_seqlen_k, int prefix_len,
+                                                       int32_t* launches);
 ACACHE_API int acache_shared_prefix_attention(const void* q, int64_t q_stride, void* out, int64_t o_stride,
                                               const void* k_cache, const void* v_cache, int64_t num_slots, int total_q,
                                               int n_heads, int n_kv_heads, int head_dim, int dtype,

@@ -55,3 +55,20 @@ def test_requests_without_queries_need_no_scratch(sizes):
 
     code = f"from acache_b200 import _lib; assert _lib.load().acache_shared_prefix_attention_scratch_bytes(*{sizes}) == 0"
     assert subprocess.run([sys.executable, "-c", code], cwd=REPO).returncode == 0
+
+
+@pytest.mark.parametrize("sizes,kernels", [
+    ((4, 4, 2, 64, 2, 0, 4, 10), 0),                   # nothing to compute
+    ((4, 4, 2, 64, 4, 1, 100, 0), 1),                  # no prefix, the own part writes the output
+    ((64, 28, 4, 128, 64, 1, 1024, 32768), 2),         # the own part merges in place
+    ((4, 4, 2, 64, 4, 1, 100000, 0), 2),               # few long ranges and their merge
+    ((1024, 28, 4, 128, 32, 32, 700, 8192), 3)])       # own rows that fill the wide tiles
+def test_the_number_of_kernels_that_a_call_launches(sizes, kernels):
+    import ctypes
+
+    from acache_b200 import _lib
+
+    lib, n = _lib.load(), ctypes.c_int32(-1)
+    nbytes = lib.acache_shared_prefix_attention_plan(*sizes, ctypes.byref(n))
+    assert n.value == kernels
+    assert nbytes == lib.acache_shared_prefix_attention_scratch_bytes(*sizes) == lib.acache_shared_prefix_attention_plan(*sizes, None)

@@ -347,3 +347,20 @@ def test_a_padded_batch_without_queries(n, batch, prefix):
             scratch.data_ptr(), nbytes, None, torch.cuda.current_stream().cuda_stream) == 0
         assert (out == 7).all()
     _lib.check_device_errors()
+
+
+@pytest.mark.parametrize("q_lens,k_lens,prefix,kernels", [([1, 1], [20, 3], 0, 1), ([1, 1], [20, 3], 300, 2), ([40, 60], [20, 300], 300, 3)])
+def test_launches_are_counted_as_they_are_made(q_lens, k_lens, prefix, kernels):
+    """The binding's count against the kernels that the profiler sees."""
+    _lib, m = _fn()
+    case = [t.to(DEV) for t in _inputs(q_lens, k_lens, prefix, 14, 2, 64, BF)[:7]]
+    kw = dict(max_seqlen_q=max(q_lens), max_seqlen_k=max(k_lens))
+    m.shared_prefix_attention(*case, **kw)
+    torch.cuda.synchronize()
+    before = _lib.LAUNCHES
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        m.shared_prefix_attention(*case, **kw)
+        torch.cuda.synchronize()
+    assert _lib.LAUNCHES - before == kernels
+    seen = [e.name for e in prof.events() if "rows_kernel" in e.name or "wide_parts_kernel" in e.name or "merge_kernel" in e.name]
+    assert len(seen) in (0, kernels), seen             # 0: no profiler on this machine
