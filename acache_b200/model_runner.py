@@ -232,10 +232,18 @@ class _DecodeGraph:
             # one memory pool for all decode graphs: they never run at the same time and the
             # logits of one replay are consumed before the next replay
             runner._graph_pool = torch.cuda.graph_pool_handle()
+        # a cyclic collection in the middle of a capture may free another runner's graph, which invalidates this one
+        collecting, stream = gc.isenabled(), torch.cuda.current_stream()
+        gc.disable()
         try:
             with torch.cuda.graph(graph, pool=runner._graph_pool):
                 self.logits = forward()
+        except BaseException:
+            torch.cuda.set_stream(stream)      # the context does not restore it when ending the capture is what failed
+            raise
         finally:
+            if collecting:
+                gc.enable()
             _lib.end_graph_capture()
         self.launches = _lib.LAUNCHES - launches0
         _lib.LAUNCHES = launches0   # nothing ran during the capture
