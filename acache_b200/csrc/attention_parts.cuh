@@ -28,6 +28,15 @@ struct Args {
 };
 
 #ifdef __CUDACC__
+// Softmax weights are rounded to the tensors' type T before their product with V, as the tensor cores take them (their sum is not
+// rounded): half a step of every weight, 1.4 (bf16) to 1.3 (fp16) times the error that the rounding of the result alone makes.
+// They are 2^(score - reference), and the reference follows the row's largest score once that is kLag above it.  fp16 numbers
+// are subnormal below 2^-14, so there the reference is kept kHead below the largest score when it is set: weights reach up to
+// 2^15 and have full precision down to 2^-21 of the largest (2^-32 of it, absolutely, below).
+template <typename T> constexpr float kHead = 0.f;
+template <> inline constexpr float kHead<__half> = 7.f;
+template <typename T> constexpr float kLag = 8.f + kHead<T>;
+
 struct Range { int q0, n_q, k0, n_k; };
 
 // rows and keys of request b, kept inside the arrays whatever the offsets say

@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(RT * NG * 32, 8 / NG) rows_kernel(const __grid
     }
 #pragma unroll
     for (int k = 0; k < NS - 1; ++k) dead_q[k] = dead_q[k + 1];
-    // ---- online softmax; O is rescaled only when a row's maximum grows by more than 2^8
+    // ---- online softmax; O is rescaled only when a row's maximum grows by more than 2^8 (attention_parts.cuh)
+    constexpr float kHead = parts::kHead<T>, kLag = parts::kLag<T>;
     float mx[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -396,12 +397,12 @@ __global__ void __launch_bounds__(RT * NG * 32, 8 / NG) rows_kernel(const __grid
       v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
       mx[h] = v * a.scale_log2;
     }
-    if (__any_sync(0xFFFFFFFFu, mx[0] > m_ref[0] + 8.f || mx[1] > m_ref[1] + 8.f)) {
+    if (__any_sync(0xFFFFFFFFu, mx[0] > m_ref[0] + kLag || mx[1] > m_ref[1] + kLag)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const bool grow = mx[h] > m_ref[h] + 8.f;
-        const float f = grow ? ex2(m_ref[h] - mx[h]) : 1.f;
-        if (grow) m_ref[h] = mx[h];
+        const bool grow = mx[h] > m_ref[h] + kLag;
+        const float f = grow ? ex2(m_ref[h] - (mx[h] - kHead)) : 1.f;
+        if (grow) m_ref[h] = mx[h] - kHead;
         l_sum[h] *= f;
 #pragma unroll
         for (int d = 0; d < D / 8; ++d) {

@@ -19,7 +19,7 @@
 // it while it looks for the tile's maximum.  When neither thread sees a score beyond 2^8 times it (one barrier with a vote
 // per tile and pair of warps says so) the weights stand; otherwise the two exchange their maxima, each rescales its half
 // of O (after P V(i-1)), and both form the weights again with the new one.  The final division by the row sum makes it
-// exact.
+// exact.  Weights are rounded to the tensors' type before P V, their sum is not (attention_parts.cuh).
 //
 // The result of a row is (O / l, log2 of its sum), fp32, turned through shared memory so that warps write whole 128-byte
 // lines.  The S and O barriers of tile i are number i & 1 of two: a waiter is never a full round of them behind, since
@@ -319,6 +319,7 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
           : "+r"(any) : "r"(pair_bar) : "memory");
       return any != 0;
     };
+    constexpr float kHead = parts::kHead<T>, kLag = parts::kLag<T>;
     float m_ref = -INFINITY, l_sum = 0.f;
     bool ok = true;
     for (int i = 0; i < n_tiles; ++i) {
@@ -389,17 +390,17 @@ wide_parts_kernel(const __grid_constant__ parts::Args a, const __grid_constant__
           weigh(xb, dh, w + 16, nm2);
           mx *= a.scale_log2;
           // does any of the 64 threads see a score beyond its row's reference (or know of a wait that ran out)?
-          if (!vote(mx > m_ref + 8.0f || bad)) break;
+          if (!vote(mx > m_ref + kLag || bad)) break;
           s_max[half * 256 + row] = mx;
           if (vote(bad)) {             // both warps leave together: neither may meet the other's barrier alone
             leave = true;
             break;
           }
           mx = fmaxf(mx, s_max[(half ^ 1) * 256 + row]);
-          const bool grow = mx > m_ref + 8.0f;
-          const float f = grow ? ex2(m_ref - mx) : 1.0f;
+          const bool grow = mx > m_ref + kLag;
+          const float f = grow ? ex2(m_ref - (mx - kHead)) : 1.0f;
           l_sum *= f;
-          if (grow) m_ref = mx;
+          if (grow) m_ref = mx - kHead;
           if (i > 0) {
             // O may only be touched between two products: P V(i-1) is done, P V(i) needs this thread's P(i)
             ok = wait_tile(BAR_O + rb * NS, i - 1) && ok;

@@ -364,3 +364,27 @@ def test_launches_are_counted_as_they_are_made(q_lens, k_lens, prefix, kernels):
     assert _lib.LAUNCHES - before == kernels
     seen = [e.name for e in prof.events() if "rows_kernel" in e.name or "wide_parts_kernel" in e.name or "merge_kernel" in e.name]
     assert len(seen) in (0, kernels), seen             # 0: no profiler on this machine
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("q_lens", [[1], [20], [120]])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_a_long_flat_tail_behind_large_weights(q_lens, where, dtype):
+    """Every 32nd key has the weight 1 and a value of 0, the others share the rest with one tiny weight: each weight is rounded by no
+    more than half a step of its own, also where fp16 numbers of its size are subnormal.  (Weights of 700.49, 100.49 and 20.49
+    steps of 2^-24: rounded on that grid they would all be off by half of one.)"""
+    _lib, m = _fn()
+    n, D = 32768, 64
+    for steps in (700.49, 100.49, 20.49):
+        low = torch.tensor(steps / 2 ** 24, dtype=torch.float64).log()
+        high = low.to(dtype).double()
+        q = torch.zeros(sum(q_lens), 2, D, dtype=dtype)
+        q[..., :2] = 8.0
+        kc, vc = torch.zeros(n // 256, 256, 1, D, dtype=dtype), torch.ones(n // 256, 256, 1, D, dtype=dtype)
+        keys, values = kc.view(-1, D), vc.view(-1, D)
+        keys[:, 0], keys[:, 1] = high, low - high      # scores (8 x + 8 y) / 8
+        keys[::32], values[::32] = 0, 0
+        slots, none = torch.arange(n, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+        pre, own = (slots, none) if where == "prefix" else (none, slots)
+        cu_q = torch.tensor([0, sum(q_lens)], dtype=torch.int32)
+        _check(m, (q, kc, vc, pre, cu_q, torch.tensor([0, own.numel()], dtype=torch.int32), own, None))
