@@ -579,9 +579,10 @@ struct Plan {
 
 // Key ranges per request.  The prefix is cut so that its CTAs fill the SMs once, into ranges of at least two tiles.  The
 // requests' own keys stay in one range, whose CTA also merges the prefix parts, unless few long ones leave most SMs idle:
-// 64 keys take a four-group CTA about 0.65 us and the merge kernel 5 us.  Measured (us): 16 requests x 32 rows x 32 heads over
-// 800 keys, own keys merged in place 66 with two prefix ranges and 69 with one, with a merge kernel 73-81; 64 tokens over
-// 32768 keys 67 with 18 ranges (72 when a merge kernel took 79 and 14 ranges 83).
+// 64 keys take a four-group CTA about 0.65 us and the merge kernel 5 us.  Fitted while the own part still ran beside the prefix
+// part (us; both came out 3-5 longer since, the choice was not fitted again): 16 requests x 32 rows x 32 heads over 800 keys, own
+// keys merged in place 66 with two prefix ranges and 69 with one, with a merge kernel 73-81; 64 tokens over 32768 keys 67 with
+// 18 ranges (72 when a merge kernel took 79 and 14 ranges 83).
 static Plan make_plan(int total_q, int batch, int max_q, int max_k, int prefix_len, int n_heads, int n_kv_heads) {
   const int64_t g = n_heads / n_kv_heads;
   if (max_q > total_q) max_q = total_q;

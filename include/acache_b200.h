@@ -369,7 +369,8 @@ ACACHE_API int acache_attention_grouped(const void* q, int64_t q_stride, void* o
  * The prefix is multiplied once with the rows of all requests; long key ranges are split.  A request without any
  * key gets zeros, a row outside every request is left as it was.  Slots outside the cache are skipped and raise
  * err_flag code 3.  max_seqlen_q / max_seqlen_k: host-known upper bounds of a request's queries and own keys.
- * softmax_scale is positive and finite, else ACACHE_EINVAL.
+ * softmax_scale is positive and finite, else ACACHE_EINVAL.  Scores, sums and O are fp32; the softmax weights are rounded to
+ * the tensors' type before their product with V, as acache_attention rounds them.
  * 16-bit dtypes, head_dim 64 or 128, 16-byte aligned rows, else ACACHE_EUNSUPPORTED; at most 2047 requests and
  * 2^23 (query, head of a group) rows, else ACACHE_ELIMIT.  scratch (16-byte aligned, contents irrelevant) holds
  * acache_shared_prefix_attention_scratch_bytes() of the same sizes and belongs to the call until it has run. */
