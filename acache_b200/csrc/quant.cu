@@ -40,7 +40,7 @@ struct Params {
   int8_t* q; float* scale; int n_rows, n_cols;
 };
 
-// silu(x) = x / (1 + e^-x) for two x down to -80 (below, e^-x leaves fp32).  e^-x is a power of two whose exponent -x log2(e) is
+// silu(x) = x / (1 + e^-x) for two |x| <= 80 (e^-x leaves fp32 below, the exponent far above).  e^-x is a power of two whose exponent -x log2(e) is
 // formed with what its rounding loses, since an error of d there is one of 0.7 d of the value: within 2^-20 of its value.  Fast
 // powers and reciprocals, two values to an instruction: expf and exact divisions made the kernel bound by instructions
 // (512 x 12288: 14 us against 8).  An infinity gives a NaN, as its row gets a NaN scale either way.
@@ -63,12 +63,16 @@ __device__ __forceinline__ float relu(float x) { return x > 0.f ? x : (x == x ? 
 // gelu(x) = x (1 + erf(x / sqrt 2)) / 2 down to -3: two steps of erff over a sum that cancels, within 2^-14 of its value
 __device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678f)); }
 
-// gates further below zero than this have forms of their own, which would cost the others a tenth (silu) to a third (gelu) more
-__device__ __forceinline__ float far_below(int act) { return act == 0 ? 80.f : (act == 1 ? INFINITY : 3.f); }
+// gates further from zero (silu) or below it (gelu) than this have forms of their own, which would cost the others a tenth (silu) to
+// a third (gelu) more
+__device__ __forceinline__ float far_limit(int act) { return act == 0 ? 80.f : (act == 1 ? INFINITY : 3.f); }
+__device__ __forceinline__ float far_of(float x, int act) { return act == 0 ? fabsf(x) : -x; }
 // silu as x e^x / (1 + e^x): within 2^-20 of its value, and 2^-149 |x| below -87, where e^x is subnormal; gelu as
 // x erfc(-x / sqrt 2) / 2: the rounding of the argument counts x^2 times, within (x^2 + 8) 2^-23 of its value
 __device__ __noinline__ float act_far(float x, int act) {
   if (act != 0) return 0.5f * x * erfcf(x * -0.70710678f);
+  if (x > 0.f) return x;
+  if (x < -128.f) return x * 0.f;                         // e^x is below all numbers, and its exponent might overflow
   const float t = x * kLog2e, rest = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -t));
   float p;
   asm("ex2.approx.f32 %0, %1;" : "=f"(p) : "f"(t));       // with subnormal results
@@ -76,17 +80,19 @@ __device__ __noinline__ float act_far(float x, int act) {
   return __fdividef(x * z, 1.f + z);
 }
 
-// y = act(gate) * up for N values; the gate furthest below zero into `far`
+// y = act(gate) * up for N values; `far` grows to the largest far_of() of the gates
 template <int N>
 __device__ __forceinline__ void gated(const float (&g)[N], const float (&u)[N], int act, float (&y)[N], float& far) {
   using namespace tc;
-#pragma unroll
-  for (int e = 0; e < N; e += 2) far = max3(far, -g[e], -g[e + 1]);
   if (act == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) far = max3(far, fabsf(g[e]), fabsf(g[e + 1]));
 #pragma unroll
     for (int e = 0; e < N; e += 2)
       unpack_f32x2(mul_f32x2(silu2(pack_f32x2(g[e], g[e + 1])), pack_f32x2(u[e], u[e + 1])), y[e], y[e + 1]);
   } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) far = max3(far, -g[e], -g[e + 1]);
 #pragma unroll
     for (int e = 0; e < N; ++e) y[e] = (act == 1 ? relu(g[e]) : gelu(g[e])) * u[e];
   }
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const P
       }
     }
     if constexpr (SRC == SRC_GATE) {
-      const float limit = far_below(p.act);
+      const float limit = far_limit(p.act);
       if (far > limit) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
@@ -271,7 +277,7 @@ __global__ void __launch_bounds__(NT, resident(NT, VPT)) quantise_kernel(const P
             b.u = next_row[(VPT + i) * NT + tid];
 #pragma unroll
             for (int e = 0; e < E; ++e)
-              if (-to_f32<T>(a.e[e]) > limit) y[i][e] = act_far(to_f32<T>(a.e[e]), p.act) * to_f32<T>(b.e[e]);
+              if (far_of(to_f32<T>(a.e[e]), p.act) > limit) y[i][e] = act_far(to_f32<T>(a.e[e]), p.act) * to_f32<T>(b.e[e]);
           }
         }
       }
@@ -392,7 +398,7 @@ __global__ void __launch_bounds__(256) quantise_any_kernel(const Params p) {
       const float u[2] = {to_f32<T>(xr[p.n_cols + c]), 0.f}, g[2] = {v, 0.f};
       float y[2], far = 0.f;
       gated<2>(g, u, p.act, y, far);
-      return far > far_below(p.act) ? act_far(v, p.act) * u[0] : y[0];
+      return far > far_limit(p.act) ? act_far(v, p.act) * u[0] : y[0];
     }
     return v;
   };

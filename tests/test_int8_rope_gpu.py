@@ -394,6 +394,24 @@ def test_gates_far_below_zero_that_make_a_row_s_largest_value(act, cols):
         _check_quantised(q[i:i + 1], s[i:i + 1], y[i:i + 1], rel)
 
 
+@pytest.mark.parametrize("cols", [64, 4096, 50, 40000])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gates_at_the_ends_of_the_range(act, cols):
+    """Finite gates up to the largest number, of either sign: the activation is the gate or zero, nothing overflows on the way."""
+    _lib, ops = _ops()
+    top = torch.finfo(BF).max
+    x = torch.randn(8, 2 * cols, generator=torch.Generator().manual_seed(cols))
+    for i, v in enumerate([top, 2.5e38, 1e30, 129.0, -129.0, -1e30, -2.5e38, -top]):
+        x[i, 3], x[i, cols + 3] = v, 0.5
+    x = x.to(BF)
+    q, s = ops.act_mul_halves_int8(x.to(DEV), act)
+    y = (_act64(x[:, :cols].double(), act) if act != "gelu" else _gelu64(x[:, :cols].double())) * x[:, cols:].double()
+    assert torch.isfinite(s).all()
+    for i in range(8):
+        # silu and gelu of gates around 0 as in their own tests; of a gate beyond 128 exact, in all rows that it decides
+        _check_quantised(q[i:i + 1], s[i:i + 1], y[i:i + 1], 2.0 ** -14 if act == "gelu" else 2.0 ** -19)
+
+
 def _gelu64(x):
     return 0.5 * x * torch.special.erfc(-x / math.sqrt(2))      # 1 + erf(x / sqrt 2) without its cancellation
 
