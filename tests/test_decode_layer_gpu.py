@@ -462,3 +462,30 @@ def test_engine_with_rope_scaling_equals_the_oracle(kind, nh, hkv, max_num_seqs,
     # the frequencies matter: the plain ones give other tokens
     monkeypatch.undo()
     assert expected()[0] != want
+
+
+@pytest.mark.parametrize("kind", ["llada", "dream"])
+def test_engine_with_stretched_frequencies_8_bits_and_the_shared_span_once(kind, monkeypatch):
+    """All three in one engine: replayed tokens equal eager ones, and the switches act (blocks in 8 bits, scaled scores)."""
+    import functools
+
+    from acache_b200 import ops
+    from acache_b200.model import configuration
+    from oracle.models import random_state_dict
+
+    scaling = dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=64)
+    for name in ("LLaDAConfig", "DreamConfig"):
+        monkeypatch.setattr(configuration, name, functools.partial(getattr(configuration, name), rope_scaling=scaling))
+    arch = _arch(kind)
+    A, G, T = 150, 16, 8
+    rng = random.Random(12)
+    affix = [rng.randint(1, 170) for _ in range(A)]
+    reqs = _random_requests(rng, arch, 5, A, G, ["prefix"], affix)
+    hf_cfg, model = (_llada if kind == "llada" else _dream)(arch, random_state_dict(arch, seed=21, std=0.2), BF)
+    eager, graphs = (_serve(model, hf_cfg, arch, kind, reqs, G, T, share_span_once=True, int8_projections=True, use_cuda_graphs=on)
+                     for on in (False, True))
+    assert graphs == eager and all(arch.mask_id not in o for o in eager)
+    blocks = model.model.transformer["blocks"] if kind == "llada" else model.model.layers
+    attn = blocks[0].attn if kind == "llada" else blocks[0].self_attn.attn
+    factor = ops.rope_frequencies(64, arch.rope_theta, scaling)[1]
+    assert blocks[0].int8 is not None and abs(attn.scale - factor ** 2 * 64 ** -0.5) < 1e-12
